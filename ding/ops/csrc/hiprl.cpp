@@ -45,6 +45,15 @@ std::vector<torch::Tensor> vtrace_bwd(
     torch::Tensor t_logit, torch::Tensor row_out, torch::Tensor value, torch::Tensor ret, torch::Tensor adv,
     torch::Tensor action, torch::Tensor weight, torch::Tensor gscales
 );
+std::vector<torch::Tensor> token_log_prob_fwd(
+    torch::Tensor logits, torch::Tensor index, double temperature, int64_t ignore, int64_t has_ignore,
+    int64_t want_entropy, int64_t top
+);
+torch::Tensor token_log_prob_bwd(
+    torch::Tensor logits, torch::Tensor index, torch::Tensor stats, torch::Tensor entropy, torch::Tensor top_index,
+    torch::Tensor grad_log_prob, torch::Tensor grad_entropy, torch::Tensor grad_top, double temperature,
+    int64_t ignore, int64_t has_ignore
+);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "DI-engine MI355X HIP kernels (gfx950)";
@@ -62,4 +71,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("conv_wrw_nhwc", &conv_wrw_nhwc, "NHWC conv2d backward-weights (fp32, register-tiled)");
     m.def("vtrace_fwd", &vtrace_fwd, "fused v-trace loss forward");
     m.def("vtrace_bwd", &vtrace_bwd, "fused v-trace loss backward");
+    m.def("token_log_prob_fwd", &token_log_prob_fwd, "token log probabilities, entropy and top alternatives");
+    m.def("token_log_prob_bwd", &token_log_prob_bwd, "gradient of token_log_prob_fwd");
 }

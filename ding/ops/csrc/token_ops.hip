@@ -1,0 +1,638 @@
+// Token log probabilities with entropy and top alternatives, forward and backward.
+//
+// For a row x of V logits, temperature T and z = x / T:
+//   lse = log sum_v exp z_v,  log p_v = z_v - lse,  H = lse - sum_v p_v z_v,
+//   top_j = log p of the j-th largest logit (equal logits: the lower index first)
+//   dx_v = 1/T [ (g_lp [v = i] + sum_j g_top_j [v = top_j]) - p_v (g_lp + sum_j g_top_j)
+//               - g_H p_v (log p_v + H) ]
+// Bound by memory: the forward reads each live logit once, the backward reads it once more and writes the gradient
+// once. Everything is kept in base 2 relative to the row's maximum: with k = log2(e) / T, d_v = (x_v - max) k,
+// s = sum 2^d, t = sum 2^d d, so log p = ln2 (d - log2 s) and H = ln2 (log2 s - t / s). All sums are 32 bit.
+//
+// A row is cut into segments of 8192 logits, one workgroup each: every thread holds 32 of them in registers, so a
+// segment is read once, also where its largest entries are wanted. The segments of a row are joined by a second,
+// small kernel; a row of one segment needs none. Rows of up to 512 entries (action sets) share a workgroup instead,
+// 16 or 64 lanes a row.
+#include "common.h"
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPerThread = 32;
+constexpr int kSegment = kThreads * kPerThread;
+constexpr int kMostTop = 32;
+constexpr int kMostJoined = 4096;  // candidates that a row's segments may offer
+constexpr float kLn2 = 0.69314718055994531f;
+// 2^-200 is zero in 32 bits: entries that far below the maximum count nothing, and 0 * -inf is kept out of the sums
+constexpr float kFar = -200.f;
+
+struct Rows {
+    const void* base;
+    int64_t inner;          // row r lies at (r / inner) * outer_stride + (r % inner) * inner_stride elements
+    int64_t outer_stride;
+    int64_t inner_stride;
+};
+
+template <typename T>
+__device__ inline const T* row_of(const Rows& rows, int64_t r) {
+    return (const T*)rows.base + (r / rows.inner) * rows.outer_stride + (r % rows.inner) * rows.inner_stride;
+}
+
+__device__ inline float to_f(float v) { return v; }
+__device__ inline float to_f(__half v) { return __half2float(v); }
+__device__ inline float to_f(__hip_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ inline T from_f(float v);
+template <> __device__ inline float from_f<float>(float v) { return v; }
+template <> __device__ inline __half from_f<__half>(float v) { return __float2half(v); }
+template <> __device__ inline __hip_bfloat16 from_f<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
+
+// 16 bytes of logits; rows of an odd length start anywhere, so the load assumes the element's alignment only
+template <typename T>
+struct Pack {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+template <typename T>
+__device__ inline Pack<T> load_pack(const T* p) {
+    Pack<T> out;
+    __builtin_memcpy(&out, p, 16);
+    return out;
+}
+template <typename T>
+__device__ inline void store_pack(T* p, const Pack<T>& v) {
+    __builtin_memcpy(p, &v, 16);
+}
+
+// A value and its index as one integer: larger values first, among equal ones the lower index. -0 equals +0; NaN sorts
+// above +inf. 0 is below every entry.
+__device__ inline unsigned long long order_of(float x, int index) {
+    int bits = __float_as_int(x + 0.f);
+    unsigned ordered = (unsigned)(bits ^ ((bits >> 31) & 0x7fffffff)) ^ 0x80000000u;
+    if (x != x) ordered = 0xffffffffu;
+    return ((unsigned long long)ordered << 32) | (unsigned)(0x7fffffff - index);
+}
+__device__ inline int index_in(unsigned long long order) { return 0x7fffffff - (int)(unsigned)order; }
+__device__ inline float value_in(unsigned long long order) {
+    unsigned ordered = (unsigned)(order >> 32) ^ 0x80000000u;
+    int bits = (int)ordered;
+    return __int_as_float(bits ^ ((bits >> 31) & 0x7fffffff));
+}
+
+struct Sums {
+    float m, s, t;
+};
+
+// sums relative to `to` instead of their own maximum
+__device__ inline void shift(Sums& a, float to, float k) {
+    float d = fmaxf((a.m - to) * k, kFar);
+    float f = __builtin_amdgcn_exp2f(d);
+    a.t = f * (a.t + d * a.s);
+    a.s = f * a.s;
+    a.m = to;
+}
+
+__device__ inline Sums join(Sums a, Sums b, float k) {
+    float m = fmaxf(a.m, b.m);
+    shift(a, m, k);
+    shift(b, m, k);
+    return {m, a.s + b.s, a.t + b.t};
+}
+
+template <int W>
+__device__ inline float group_max(float v) {
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, W));
+    return v;
+}
+template <int W>
+__device__ inline float group_sum(float v) {
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, W);
+    return v;
+}
+template <int W>
+__device__ inline unsigned long long group_max(unsigned long long v) {
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+        unsigned long long u = __shfl_xor(v, o, W);
+        v = u > v ? u : v;
+    }
+    return v;
+}
+
+struct Out {
+    float* log_prob;      // [rows]
+    float* entropy;       // [rows] or null
+    float* stats;         // [rows, 2]: maximum, log2 s
+    float* top_log_prob;  // [rows, top]
+    int64_t* top_index;   // [rows, top]
+};
+
+__device__ inline float log2_of(float s) { return __builtin_amdgcn_logf(s); }
+
+// what one lane writes for a row whose sums are known
+template <typename T>
+__device__ inline void write_row(const Out& out, int64_t r, Sums a, const T* x, int64_t token, int V, float k) {
+    float log2s = log2_of(a.s);
+    float lp = __builtin_nanf("");
+    if (token >= 0 && token < V) lp = ((to_f(x[token]) - a.m) * k - log2s) * kLn2;
+    out.log_prob[r] = lp;
+    if (out.entropy) out.entropy[r] = (log2s - a.t / a.s) * kLn2;
+    out.stats[2 * r] = a.m;
+    out.stats[2 * r + 1] = log2s;
+}
+
+__device__ inline void write_top(const Out& out, int64_t r, int top, int j, unsigned long long order, float m,
+                                 float log2s, float k) {
+    out.top_log_prob[r * top + j] = ((value_in(order) - m) * k - log2s) * kLn2;
+    out.top_index[r * top + j] = index_in(order);
+}
+
+__device__ inline void write_nothing(const Out& out, int64_t r, int top, int lane, int lanes) {
+    if (lane == 0) {
+        out.log_prob[r] = 0.f;
+        if (out.entropy) out.entropy[r] = 0.f;
+        out.stats[2 * r] = 0.f;
+        out.stats[2 * r + 1] = 0.f;
+    }
+    for (int j = lane; j < top; j += lanes) {
+        out.top_log_prob[r * top + j] = 0.f;
+        out.top_index[r * top + j] = -1;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- short rows, forward
+// LANES lanes hold a row in registers, PER entries each.
+template <typename T, int LANES, int PER>
+__global__ void __launch_bounds__(kThreads) token_short_fwd(
+    Rows rows, const int64_t* __restrict__ index, Out out, int64_t count, int V, float k, int64_t ignore,
+    int has_ignore, int top
+) {
+    int lane = threadIdx.x % LANES;
+    int64_t r = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+    if (r >= count) return;
+    int64_t token = index[r];
+    if (has_ignore && token == ignore) {
+        write_nothing(out, r, top, lane, LANES);
+        return;
+    }
+    const T* x = row_of<T>(rows, r);
+    float v[PER];
+    Sums a{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        int c = j * LANES + lane;
+        v[j] = c < V ? to_f(x[c]) : -INFINITY;
+        a.m = fmaxf(a.m, v[j]);
+    }
+    a.m = group_max<LANES>(a.m);
+    float ref = a.m == -INFINITY ? 0.f : a.m;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        float d = (v[j] - ref) * k;
+        float e = __builtin_amdgcn_exp2f(d);
+        a.s += e;
+        a.t += e * fmaxf(d, kFar);
+    }
+    a.s = group_sum<LANES>(a.s);
+    a.t = group_sum<LANES>(a.t);
+    if (lane == 0) write_row(out, r, a, x, token, V, k);
+    float log2s = log2_of(a.s);
+    unsigned long long below = ~0ull;
+    for (int j = 0; j < top; ++j) {
+        unsigned long long best = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            int c = i * LANES + lane;
+            unsigned long long o = c < V ? order_of(v[i], c) : 0;
+            if (o < below && o > best) best = o;
+        }
+        below = group_max<LANES>(best);
+        if (lane == 0) write_top(out, r, top, j, below, a.m, log2s, k);
+    }
+}
+
+// ----------------------------------------------------------------------------------------------- long rows, forward
+
+// `top` largest of n orders in LDS, in descending order: each one's place is the number of larger ones
+template <typename F>
+__device__ inline void rank_orders(const unsigned long long* orders, int n, int top, F&& put) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        unsigned long long mine = orders[i];
+        if (mine == 0) continue;
+        int larger = 0;
+        for (int j = 0; j < n && larger < top; ++j) larger += orders[j] > mine;
+        if (larger < top) put(larger, mine);
+    }
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_segment_fwd(
+    Rows rows, const int64_t* __restrict__ index, Out out, int V, int segments, float k, int64_t ignore,
+    int has_ignore, int top, float* __restrict__ partial, unsigned long long* __restrict__ offered
+) {
+    constexpr int N = Pack<T>::N;
+    int64_t r = blockIdx.x / segments;
+    int seg = blockIdx.x % segments;
+    int tid = threadIdx.x;
+    int64_t token = index[r];
+    if (has_ignore && token == ignore) {
+        if (seg == 0) write_nothing(out, r, top, tid, kThreads);
+        return;
+    }
+    const T* x = row_of<T>(rows, r);
+    int lo = seg * kSegment;
+    Pack<T> v[kPerThread / N];
+#pragma unroll
+    for (int j = 0; j < kPerThread / N; ++j) {
+        int c = lo + (j * kThreads + tid) * N;
+        if (c + N <= V) {
+            v[j] = load_pack(x + c);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[j].v[i] = c + i < V ? x[c + i] : from_f<T>(-INFINITY);
+        }
+    }
+    Sums a{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kPerThread / N; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) a.m = fmaxf(a.m, to_f(v[j].v[i]));
+    a.m = group_max<kWave>(a.m);
+    float ref = a.m == -INFINITY ? 0.f : a.m;
+#pragma unroll
+    for (int j = 0; j < kPerThread / N; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float d = (to_f(v[j].v[i]) - ref) * k;
+            float e = __builtin_amdgcn_exp2f(d);
+            a.s += e;
+            a.t += e * fmaxf(d, kFar);
+        }
+    a.s = group_sum<kWave>(a.s);
+    a.t = group_sum<kWave>(a.t);
+    __shared__ Sums part[kThreads / kWave];
+    if (tid % kWave == 0) part[tid / kWave] = a;
+
+    // Largest entries. Of the threads' own largest, the top-th is a bound that all wanted entries reach, and only
+    // `top` threads hold entries that reach it: at most top * kPerThread candidates.
+    __shared__ unsigned long long best[TOP ? kThreads : 1];
+    __shared__ unsigned long long bound_s;
+    __shared__ unsigned long long candidates[TOP ? kMostTop * kPerThread : 1];
+    __shared__ int found;
+    if constexpr (TOP) {
+        unsigned long long mine = 0;
+#pragma unroll
+        for (int j = 0; j < kPerThread / N; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                int c = lo + (j * kThreads + tid) * N + i;
+                unsigned long long o = c < V ? order_of(to_f(v[j].v[i]), c) : 0;
+                mine = o > mine ? o : mine;
+            }
+        best[tid] = mine;
+        if (tid == 0) {
+            bound_s = 1;  // fewer than `top` threads hold entries: all of theirs are candidates
+            found = 0;
+        }
+        __syncthreads();
+        int larger = 0;
+        for (int j = 0; j < kThreads; ++j) larger += best[j] > mine;
+        if (mine != 0 && larger == top - 1) bound_s = mine;
+        __syncthreads();
+        unsigned long long bound = bound_s;
+#pragma unroll
+        for (int j = 0; j < kPerThread / N; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                int c = lo + (j * kThreads + tid) * N + i;
+                unsigned long long o = c < V ? order_of(to_f(v[j].v[i]), c) : 0;
+                if (o >= bound) candidates[atomicAdd(&found, 1)] = o;
+            }
+    }
+    __syncthreads();
+    Sums all = part[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / kWave; ++w) all = join(all, part[w], k);
+    if (segments == 1) {
+        if (tid == 0) write_row(out, r, all, x, token, V, k);
+        if constexpr (TOP) {
+            float log2s = log2_of(all.s);
+            rank_orders(candidates, found, top, [&](int j, unsigned long long o) {
+                write_top(out, r, top, j, o, all.m, log2s, k);
+            });
+        }
+    } else {
+        if (tid == 0) {
+            float* p = partial + 3 * (int64_t)blockIdx.x;
+            p[0] = all.m;
+            p[1] = all.s;
+            p[2] = all.t;
+        }
+        if constexpr (TOP) {
+            unsigned long long* mine = offered + (int64_t)blockIdx.x * top;
+            for (int j = tid; j < top; j += kThreads)
+                if (j >= found) mine[j] = 0;
+            rank_orders(candidates, found, top, [&](int j, unsigned long long o) { mine[j] = o; });
+        }
+    }
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_join(
+    Rows rows, const int64_t* __restrict__ index, Out out, int64_t count, int V, int segments, float k,
+    int64_t ignore, int has_ignore, int top, const float* __restrict__ partial,
+    const unsigned long long* __restrict__ offered
+) {
+    // with largest entries a workgroup joins one row, else each of its waves does
+    int lane = threadIdx.x % kWave;
+    int64_t r = TOP ? blockIdx.x : (int64_t)blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave;
+    if (r >= count) return;
+    int64_t token = index[r];
+    if (has_ignore && token == ignore) return;
+    Sums a{-INFINITY, 0.f, 0.f};
+    for (int g = lane; g < segments; g += kWave) {
+        const float* p = partial + 3 * (r * segments + g);
+        a = join(a, Sums{p[0], p[1], p[2]}, k);
+    }
+    float m = group_max<kWave>(a.m);
+    shift(a, m, k);
+    a.s = group_sum<kWave>(a.s);
+    a.t = group_sum<kWave>(a.t);
+    if (TOP ? threadIdx.x == 0 : lane == 0) write_row(out, r, a, row_of<T>(rows, r), token, V, k);
+    if constexpr (TOP) {
+        __shared__ unsigned long long orders[kMostJoined];
+        int n = segments * top;
+        for (int i = threadIdx.x; i < n; i += kThreads) orders[i] = offered[r * n + i];
+        __syncthreads();
+        float log2s = log2_of(a.s);
+        rank_orders(orders, n, top, [&](int j, unsigned long long o) { write_top(out, r, top, j, o, a.m, log2s, k); });
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------- backward
+
+struct Grads {
+    const float* log_prob;  // [rows] or null
+    const float* entropy;   // [rows] or null
+    const float* top;       // [rows, top] or null
+    const float* stats;
+    const float* h;         // [rows]: the entropy itself, where its gradient is given
+    const int64_t* top_index;
+};
+
+// what a row's gradient is made of: dx_v = p_v (c0 + c1 log2 p_v) + [v is one of the row's tokens] its own share
+struct RowGrad {
+    float m, log2s, c0, c1;
+};
+
+__device__ inline RowGrad row_grad(const Grads& g, int64_t r, int top, int64_t token, int V, float inv_t) {
+    RowGrad a{g.stats[2 * r], g.stats[2 * r + 1], 0.f, 0.f};
+    float sum = 0.f;
+    if (g.log_prob) {
+        sum = g.log_prob[r];
+        if (token < 0 || token >= V) sum = __builtin_nanf("");
+    }
+    if (g.top)
+        for (int j = 0; j < top; ++j) sum += g.top[r * top + j];
+    a.c0 = -sum * inv_t;
+    if (g.entropy) {
+        float ge = g.entropy[r] * inv_t;
+        a.c0 -= ge * g.h[r];
+        a.c1 = -ge * kLn2;
+    }
+    return a;
+}
+
+__device__ inline float grad_at(const RowGrad& a, float x, float k) {
+    float d = (x - a.m) * k - a.log2s;
+    return __builtin_amdgcn_exp2f(d) * (a.c0 + a.c1 * fmaxf(d, kFar));
+}
+
+// the share of column c alone, and whether lane j is the one that adds it: lanes 0..top-1 stand for the largest
+// entries, lane `top` for the token where it is none of them
+__device__ inline bool own_share(const Grads& g, int64_t r, int top, int j, int64_t token, int V, float inv_t,
+                                 int& column, float& share) {
+    bool valid = g.log_prob && token >= 0 && token < V;
+    float glp = valid ? g.log_prob[r] : 0.f;
+    if (j < top && g.top) {
+        column = (int)g.top_index[r * top + j];
+        share = (g.top[r * top + j] + (valid && column == token ? glp : 0.f)) * inv_t;
+        return true;
+    }
+    if (j == top && valid) {
+        if (g.top)
+            for (int i = 0; i < top; ++i)
+                if (g.top_index[r * top + i] == token) return false;
+        column = (int)token;
+        share = glp * inv_t;
+        return true;
+    }
+    return false;
+}
+
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads) token_short_bwd(
+    Rows rows, const int64_t* __restrict__ index, Grads g, T* __restrict__ grad, int64_t count, int V, float k,
+    float inv_t, int64_t ignore, int has_ignore, int top
+) {
+    int lane = threadIdx.x % LANES;
+    int64_t r = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+    if (r >= count) return;
+    int64_t token = index[r];
+    T* out = grad + r * V;
+    if (has_ignore && token == ignore) {
+        for (int c = lane; c < V; c += LANES) out[c] = from_f<T>(0.f);
+        return;
+    }
+    const T* x = row_of<T>(rows, r);
+    RowGrad a = row_grad(g, r, top, token, V, inv_t);
+    for (int c = lane; c < V; c += LANES) {
+        float v = grad_at(a, to_f(x[c]), k);
+        for (int j = 0; j <= top; ++j) {
+            int column;
+            float share;
+            if (own_share(g, r, top, j, token, V, inv_t, column, share) && column == c) v += share;
+        }
+        out[c] = from_f<T>(v);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) token_segment_bwd(
+    Rows rows, const int64_t* __restrict__ index, Grads g, T* __restrict__ grad, int V, int segments, float k,
+    float inv_t, int64_t ignore, int has_ignore, int top
+) {
+    constexpr int N = Pack<T>::N;
+    int64_t r = blockIdx.x / segments;
+    int lo = (blockIdx.x % segments) * kSegment;
+    int tid = threadIdx.x;
+    int64_t token = index[r];
+    T* out = grad + r * V;
+    bool live = !(has_ignore && token == ignore);
+    const T* x = row_of<T>(rows, r);
+    RowGrad a{0.f, 0.f, 0.f, 0.f};
+    if (live) a = row_grad(g, r, top, token, V, inv_t);
+#pragma unroll
+    for (int j = 0; j < kPerThread / N; ++j) {
+        int c = lo + (j * kThreads + tid) * N;
+        if (c + N <= V) {
+            Pack<T> v, o;
+            if (live) v = load_pack(x + c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) o.v[i] = from_f<T>(live ? grad_at(a, to_f(v.v[i]), k) : 0.f);
+            store_pack(out + c, o);
+        } else {
+            for (int i = 0; c + i < V; ++i) out[c + i] = from_f<T>(live ? grad_at(a, to_f(x[c + i]), k) : 0.f);
+        }
+    }
+    if (!live) return;
+    __syncthreads();  // the single columns are written again, whole, after the others
+    int column;
+    float share;
+    if (tid <= top && own_share(g, r, top, tid, token, V, inv_t, column, share) && column >= lo &&
+        column < lo + kSegment)
+        out[column] = from_f<T>(grad_at(a, to_f(x[column]), k) + share);
+}
+
+// ------------------------------------------------------------------------------------------------------------- host
+
+Rows rows_of(const torch::Tensor& logits) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 3 && (logits.stride(2) == 1 || logits.size(2) == 1),
+                "token_log_prob: logits must be [outer, inner, V] on a HIP device with unit stride along V");
+    return {logits.data_ptr(), logits.size(1), logits.stride(0), logits.stride(1)};
+}
+
+void check_index(const torch::Tensor& logits, const torch::Tensor& index) {
+    TORCH_CHECK(index.is_cuda() && index.device() == logits.device() && index.is_contiguous() &&
+                    index.scalar_type() == torch::kInt64 && index.numel() == logits.size(0) * logits.size(1),
+                "token_log_prob: index must be contiguous int64, one for each row, on the logits' device");
+    TORCH_CHECK(logits.size(2) >= 1 && logits.size(2) <= (1 << 30), "token_log_prob: V must be in [1, 2^30]");
+}
+
+template <typename F>
+void by_type(const torch::Tensor& x, F&& f) {
+    switch (x.scalar_type()) {
+        case torch::kFloat32: f((float*)nullptr); break;
+        case torch::kFloat16: f((__half*)nullptr); break;
+        case torch::kBFloat16: f((__hip_bfloat16*)nullptr); break;
+        default: TORCH_CHECK(false, "expected float32, float16 or bfloat16");
+    }
+}
+
+}  // namespace
+
+std::vector<torch::Tensor> token_log_prob_fwd(
+    torch::Tensor logits, torch::Tensor index, double temperature, int64_t ignore, int64_t has_ignore,
+    int64_t want_entropy, int64_t top
+) {
+    Rows rows = rows_of(logits);
+    check_index(logits, index);
+    c10::OptionalDeviceGuard guard(logits.device());
+    int64_t count = index.numel();
+    int V = (int)logits.size(2);
+    int segments = cdiv(V, kSegment);
+    TORCH_CHECK(top >= 0 && top <= kMostTop && top <= V, "token_log_prob: top_k must be at most ", kMostTop, " and V");
+    TORCH_CHECK(top * segments <= kMostJoined, "token_log_prob: top_k of ", top, " over ", V, " entries is too much");
+    auto opt = logits.options().dtype(torch::kFloat32);
+    auto log_prob = torch::empty({count}, opt);
+    auto entropy = torch::empty({want_entropy ? count : 0}, opt);
+    auto stats = torch::empty({count, 2}, opt);
+    auto top_log_prob = torch::empty({count, top}, opt);
+    auto top_index = torch::empty({count, top}, opt.dtype(torch::kInt64));
+    std::vector<torch::Tensor> result{log_prob, entropy, stats, top_log_prob, top_index};
+    if (count == 0) return result;
+    TORCH_CHECK(count * segments < (int64_t)1 << 31, "token_log_prob: too many rows");
+    Out out{log_prob.data_ptr<float>(), want_entropy ? entropy.data_ptr<float>() : nullptr, stats.data_ptr<float>(),
+            top_log_prob.data_ptr<float>(), top_index.data_ptr<int64_t>()};
+    float k = (float)(1.4426950408889634 / temperature);
+    hipStream_t stream = ding_current_stream();
+    const int64_t* ix = index.data_ptr<int64_t>();
+    by_type(logits, [&](auto* null) {
+        using T = std::remove_pointer_t<decltype(null)>;
+        if (V <= 64) {
+            token_short_fwd<T, 16, 4><<<cdiv(count, kThreads / 16), kThreads, 0, stream>>>(
+                rows, ix, out, count, V, k, ignore, has_ignore, top);
+        } else if (V <= 512) {
+            token_short_fwd<T, 64, 8><<<cdiv(count, kThreads / 64), kThreads, 0, stream>>>(
+                rows, ix, out, count, V, k, ignore, has_ignore, top);
+        } else {
+            torch::Tensor partial, offered;
+            float* p = nullptr;
+            unsigned long long* o = nullptr;
+            if (segments > 1) {
+                partial = torch::empty({count * segments * 3}, opt);
+                p = partial.data_ptr<float>();
+                if (top > 0) {
+                    offered = torch::empty({count * segments * top}, opt.dtype(torch::kInt64));
+                    o = (unsigned long long*)offered.data_ptr<int64_t>();
+                }
+            }
+            dim3 grid((unsigned)(count * segments));
+            if (top > 0)
+                token_segment_fwd<T, true><<<grid, kThreads, 0, stream>>>(
+                    rows, ix, out, V, segments, k, ignore, has_ignore, top, p, o);
+            else
+                token_segment_fwd<T, false><<<grid, kThreads, 0, stream>>>(
+                    rows, ix, out, V, segments, k, ignore, has_ignore, top, p, o);
+            if (segments > 1) {
+                HIP_CHECK_LAST();
+                if (top > 0)
+                    token_join<T, true><<<(unsigned)count, kThreads, 0, stream>>>(
+                        rows, ix, out, count, V, segments, k, ignore, has_ignore, top, p, o);
+                else
+                    token_join<T, false><<<cdiv(count, kThreads / kWave), kThreads, 0, stream>>>(
+                        rows, ix, out, count, V, segments, k, ignore, has_ignore, top, p, o);
+            }
+        }
+    });
+    HIP_CHECK_LAST();
+    return result;
+}
+
+torch::Tensor token_log_prob_bwd(
+    torch::Tensor logits, torch::Tensor index, torch::Tensor stats, torch::Tensor entropy, torch::Tensor top_index,
+    torch::Tensor grad_log_prob, torch::Tensor grad_entropy, torch::Tensor grad_top, double temperature,
+    int64_t ignore, int64_t has_ignore
+) {
+    Rows rows = rows_of(logits);
+    check_index(logits, index);
+    c10::OptionalDeviceGuard guard(logits.device());
+    int64_t count = index.numel();
+    int V = (int)logits.size(2);
+    int segments = cdiv(V, kSegment);
+    int top = grad_top.numel() ? (int)top_index.size(1) : 0;
+    // an empty tensor stands for a gradient that is not there
+    auto given = [&](const torch::Tensor& t, int64_t n) -> const float* {
+        if (t.numel() == 0) return nullptr;
+        TORCH_CHECK(t.device() == logits.device() && t.is_contiguous() && t.scalar_type() == torch::kFloat32 &&
+                        t.numel() == n, "token_log_prob: a gradient has another shape, type or device");
+        return t.data_ptr<float>();
+    };
+    auto grad = torch::empty(logits.sizes(), logits.options());
+    if (grad.numel() == 0) return grad;
+    TORCH_CHECK(count * segments < (int64_t)1 << 31, "token_log_prob: too many rows");
+    Grads g{given(grad_log_prob, count), given(grad_entropy, count), given(grad_top, count * top),
+            given(stats, 2 * count), given(entropy, count), top ? top_index.data_ptr<int64_t>() : nullptr};
+    TORCH_CHECK(g.stats && (g.h || !g.entropy), "token_log_prob: what the forward pass kept is missing");
+    float k = (float)(1.4426950408889634 / temperature), inv_t = (float)(1.0 / temperature);
+    hipStream_t stream = ding_current_stream();
+    const int64_t* ix = index.data_ptr<int64_t>();
+    by_type(logits, [&](auto* null) {
+        using T = std::remove_pointer_t<decltype(null)>;
+        T* to = (T*)grad.data_ptr();
+        if (V <= 64)
+            token_short_bwd<T, 16><<<cdiv(count, kThreads / 16), kThreads, 0, stream>>>(
+                rows, ix, g, to, count, V, k, inv_t, ignore, has_ignore, top);
+        else if (V <= 512)
+            token_short_bwd<T, 64><<<cdiv(count, kThreads / 64), kThreads, 0, stream>>>(
+                rows, ix, g, to, count, V, k, inv_t, ignore, has_ignore, top);
+        else
+            token_segment_bwd<T><<<(unsigned)(count * segments), kThreads, 0, stream>>>(
+                rows, ix, g, to, V, segments, k, inv_t, ignore, has_ignore, top);
+    });
+    HIP_CHECK_LAST();
+    return grad;
+}

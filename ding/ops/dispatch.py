@@ -338,3 +338,51 @@ class _WrwConv2dFn(torch.autograd.Function):
 def wrw_conv2d(x, weight, bias, stride):
     """conv2d(x, w, b, stride) with the hand-written NHWC wrw backward."""
     return _WrwConv2dFn.apply(x, weight, bias, stride)
+
+
+class _TokenLogProb(torch.autograd.Function):
+    """Token log probabilities of [outer, inner, V] logits: one pass over the
+    logits forward, one pass and one write backward. Rows keep their maximum
+    and log-sum (8 bytes) for the backward pass, not their probabilities."""
+
+    @staticmethod
+    def forward(ctx, logits, index, temperature, ignore_index, entropy, top_k):
+        ext = _load()
+        ignore = 0 if ignore_index is None else int(ignore_index)
+        log_prob, h, stats, top_log_prob, top_index = ext.token_log_prob_fwd(
+            logits, index, temperature, ignore, int(ignore_index is not None), int(entropy), top_k
+        )
+        ctx.save_for_backward(logits, index, stats, h, top_index)
+        ctx.temperature, ctx.ignore_index, ctx.ignore = temperature, ignore_index, ignore
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(top_index)
+        return log_prob, h, top_log_prob, top_index
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_log_prob, g_entropy, g_top, _):
+        logits, index, stats, h, top_index = ctx.saved_tensors
+        none = stats.new_empty(0)
+        grads = [none if g is None else g.contiguous() for g in (g_log_prob, g_entropy, g_top)]
+        grad = _load().token_log_prob_bwd(
+            logits, index, stats, h, top_index, *grads, ctx.temperature, ctx.ignore, int(ctx.ignore_index is not None)
+        )
+        return grad, None, None, None, None, None
+
+
+def token_log_prob(logits, index, temperature: float, ignore_index: Optional[int], entropy: bool, top_k: int):
+    """logits [..., V], index [...] -> (log_prob, entropy or None,
+    top_log_prob or None, top_index or None), the first three in float32."""
+    shape, V = index.shape, logits.shape[-1]
+    if logits.stride(-1) != 1:
+        logits = logits.contiguous()
+    if logits.dim() < 3:
+        logits3 = logits.reshape(1, -1, V)
+    else:
+        logits3 = logits if logits.dim() == 3 else logits.flatten(0, -3)
+    args = (logits3, index.long().contiguous(), float(temperature), ignore_index, entropy, top_k)
+    log_prob, h, top_log_prob, top_index = _TokenLogProb.apply(*args)
+    return (
+        log_prob.view(shape), h.view(shape) if entropy else None,
+        top_log_prob.view(*shape, top_k) if top_k else None, top_index.view(*shape, top_k) if top_k else None
+    )

@@ -38,4 +38,6 @@ from .sampler import (
     ArgmaxSampler, MultinomialSampler, MuSampler, ReparameterizationSampler, HybridStochasticSampler,
     HybridDeterminsticSampler,
 )
-from .log_prob_utils import naive_method, efficient_method, less_efficient_method
+from .log_prob_utils import (
+    naive_method, efficient_method, less_efficient_method, fused_method, token_log_prob, token_log_prob_output,
+)

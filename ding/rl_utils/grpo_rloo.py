@@ -4,6 +4,7 @@ Parity: reference ding/rl_utils/grpo.py:10 and rloo.py:10. Token-level
 shapes: logits [B, S, V], action [B, S].
 """
 from collections import namedtuple
+from typing import Callable
 
 import torch
 
@@ -20,15 +21,18 @@ def _token_logp(logit: torch.Tensor, action: torch.Tensor) -> torch.Tensor:
     return logp.gather(-1, action.unsqueeze(-1)).squeeze(-1)
 
 
-def grpo_policy_error(data: namedtuple, clip_ratio: float = 0.2, beta: float = 0.1):
+def grpo_policy_error(data: namedtuple, clip_ratio: float = 0.2, beta: float = 0.1,
+                      log_prob_fn: Callable = _token_logp):
     """Clipped PPO surrogate per token + beta * k3-KL to a reference policy.
-    adv is the per-sequence group-normalized advantage [B]."""
+    adv is the per-sequence group-normalized advantage [B]. ``log_prob_fn``
+    (logits, action) -> log probabilities: ``fused_method`` reads each logits
+    tensor once on a GPU."""
     logit_new, logit_old, logit_ref, action, adv, weight = data
     if weight is None:
         weight = torch.ones_like(action, dtype=logit_new.dtype)
-    logp_new = _token_logp(logit_new, action)
-    logp_old = _token_logp(logit_old, action)
-    logp_ref = _token_logp(logit_ref, action)
+    logp_new = log_prob_fn(logit_new, action)
+    logp_old = log_prob_fn(logit_old, action)
+    logp_ref = log_prob_fn(logit_ref, action)
     ratio = torch.exp(logp_new - logp_old)
     adv_tok = adv.unsqueeze(-1)  # broadcast over sequence
     surr1 = ratio * adv_tok
@@ -44,17 +48,18 @@ def grpo_policy_error(data: namedtuple, clip_ratio: float = 0.2, beta: float = 0
     return grpo_loss_tuple(policy_loss), grpo_info(approx_kl, clipfrac)
 
 
-def rloo_policy_error(data: namedtuple, clip_ratio: float = 0.2):
+def rloo_policy_error(data: namedtuple, clip_ratio: float = 0.2, log_prob_fn: Callable = _token_logp):
     """REINFORCE leave-one-out: reward [K, B_group] -> per-sample baseline is
-    the mean of the other K-1 samples; then a clipped PPO surrogate."""
+    the mean of the other K-1 samples; then a clipped PPO surrogate.
+    ``log_prob_fn`` as in ``grpo_policy_error``."""
     logit_new, logit_old, action, reward, weight = data
     if weight is None:
         weight = torch.ones_like(action, dtype=logit_new.dtype)
     K = reward.shape[0]
     baseline = (reward.sum(0, keepdim=True) - reward) / max(K - 1, 1)
     adv = (reward - baseline).reshape(-1)  # flatten to [B]
-    logp_new = _token_logp(logit_new, action)
-    logp_old = _token_logp(logit_old, action)
+    logp_new = log_prob_fn(logit_new, action)
+    logp_old = log_prob_fn(logit_old, action)
     ratio = torch.exp(logp_new - logp_old)
     adv_tok = adv.unsqueeze(-1)
     surr1 = ratio * adv_tok
