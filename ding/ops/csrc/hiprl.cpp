@@ -54,6 +54,11 @@ torch::Tensor token_log_prob_bwd(
     torch::Tensor grad_log_prob, torch::Tensor grad_entropy, torch::Tensor grad_top, double temperature,
     int64_t ignore, int64_t has_ignore
 );
+std::vector<torch::Tensor> linrec_fwd(torch::Tensor x, torch::Tensor gate, torch::Tensor h0, torch::Tensor reset);
+std::vector<torch::Tensor> linrec_bwd(
+    torch::Tensor x, torch::Tensor gate, torch::Tensor reset, torch::Tensor starts, torch::Tensor grad_h,
+    torch::Tensor grad_last, int64_t want_h0
+);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "DI-engine MI355X HIP kernels (gfx950)";
@@ -73,4 +78,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("vtrace_bwd", &vtrace_bwd, "fused v-trace loss backward");
     m.def("token_log_prob_fwd", &token_log_prob_fwd, "token log probabilities, entropy and top alternatives");
     m.def("token_log_prob_bwd", &token_log_prob_bwd, "gradient of token_log_prob_fwd");
+    m.def("linrec_fwd", &linrec_fwd, "gated linear recurrence forward");
+    m.def("linrec_bwd", &linrec_bwd, "gated linear recurrence backward");
 }

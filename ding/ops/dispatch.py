@@ -386,3 +386,40 @@ def token_log_prob(logits, index, temperature: float, ignore_index: Optional[int
         log_prob.view(shape), h.view(shape) if entropy else None,
         top_log_prob.view(*shape, top_k) if top_k else None, top_index.view(*shape, top_k) if top_k else None
     )
+
+
+class _GatedLinearRecurrence(torch.autograd.Function):
+    """h_t = r_t a_t h_{t-1} + (1 - a_t) x_t over [T, B, D]. The backward pass
+    computes the states again from 32-bit starting states that the forward
+    pass keeps, so the rounded outputs are not read."""
+
+    @staticmethod
+    def forward(ctx, x, gate, h0, reset):
+        none = x.new_empty(0)
+        start = none if h0 is None else h0.float().contiguous()
+        mask = none if reset is None else reset
+        h, last, starts = _load().linrec_fwd(x, gate, start, mask)
+        ctx.save_for_backward(x, gate, mask, starts)
+        ctx.h0_dtype = None if h0 is None else h0.dtype
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_h, g_last):
+        x, gate, mask, starts = ctx.saved_tensors
+        none = x.new_empty(0)
+        want_h0 = ctx.h0_dtype is not None and ctx.needs_input_grad[2]
+        dx, dgate, dh0 = _load().linrec_bwd(
+            x, gate, mask, starts, none if g_h is None else g_h.contiguous(),
+            none if g_last is None else g_last.contiguous(), int(want_h0)
+        )
+        return dx, dgate, dh0.to(ctx.h0_dtype) if want_h0 else None, None
+
+
+def gated_linear_recurrence(x, gate, h0, reset):
+    """x, gate [T, B, D], h0 [B, D] or None, reset [T, B] bool or None ->
+    (h [T, B, D] in x's type, last state [B, D] in float32)."""
+    x = x if x.stride(-1) == 1 else x.contiguous()
+    gate = gate if gate.stride(-1) == 1 else gate.contiguous()
+    return _GatedLinearRecurrence.apply(x, gate, h0, None if reset is None else reset.contiguous())

@@ -3,7 +3,9 @@ from .nn_module import (
     build_activation, build_normalization, sequential_pack, normed_linear, normed_conv2d, Lambda, weight_init_,
 )
 from .res_block import ResBlock, ResFCBlock
-from .rnn import LSTM, PytorchLSTM, GRU, get_lstm, sequence_mask, LSTMForwardWrapper
+from .rnn import (
+    LSTM, PytorchLSTM, GRU, GatedLinearRNN, gated_linear_recurrence, get_lstm, sequence_mask, LSTMForwardWrapper,
+)
 from .transformer import Transformer, TransformerLayer, Attention, ScaledDotProductAttention
 from .gtrxl import GTrXL, GRUGatingUnit, PositionalEmbedding, AttentionXL, Memory
 from .scatter_connection import ScatterConnection

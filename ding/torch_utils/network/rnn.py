@@ -12,6 +12,7 @@ from typing import List, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from ding.torch_utils.data_helper import zeros_like
 
@@ -189,6 +190,100 @@ class GRU(nn.GRUCell, LSTMForwardWrapper):
         return x, self._after_forward(next_state, list_next_state)
 
 
+def _gated_linear_recurrence_torch(x, gate, h0, reset):
+    dtype = torch.float64 if x.dtype == torch.float64 else torch.float32
+    x32, f = x.to(dtype), gate.to(dtype)
+    # through the logarithm, so that the gradient a (1 - a) keeps its relative precision where a is near 1
+    keep, add = F.logsigmoid(f).exp(), F.logsigmoid(-f).exp() * x32
+    h = x32.new_zeros(x.shape[1:]) if h0 is None else h0.to(dtype)
+    outputs = []
+    for t in range(x.shape[0]):
+        if reset is not None:
+            h = h.masked_fill(reset[t].unsqueeze(-1), 0.)
+        h = keep[t] * h + add[t]
+        outputs.append(h)
+    return torch.stack(outputs).to(x.dtype), h
+
+
+def gated_linear_recurrence(
+        x: torch.Tensor,
+        gate: torch.Tensor,
+        h0: Optional[torch.Tensor] = None,
+        reset: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """
+    Overview:
+        The recurrence ``h[t] = a[t] * h[t-1] + (1 - a[t]) * x[t]`` with ``a = sigmoid(gate)``, along the time of each
+        channel. It is linear in the state, so long sequences are scanned in parallel (HIP kernels,
+        ding/ops/csrc/linrec_ops.hip); a sequence of one step serves a collector. Differentiable (once).
+    Arguments:
+        - x (:obj:`torch.Tensor`): [T, B, D] of float32, bfloat16 or float16, T >= 1. Time and batch may have any \
+            strides, as a part of a larger projection has.
+        - gate (:obj:`torch.Tensor`): Like ``x``, before the sigmoid.
+        - h0 (:obj:`Optional[torch.Tensor]`): [B, D], the state before the first step; zeros by default.
+        - reset (:obj:`Optional[torch.Tensor]`): [T, B] of bool, true where an episode starts: the state before that \
+            step counts as zero.
+    Returns:
+        - h (:obj:`torch.Tensor`): [T, B, D] in ``x``'s type.
+        - last (:obj:`torch.Tensor`): [B, D], the state after the last step, in float32 (float64 for float64 inputs, \
+            which are taken on the CPU only).
+    """
+    if x.dim() != 3 or x.shape[0] < 1:
+        raise ValueError(f"x must be [T, B, D] with T >= 1, got {tuple(x.shape)}")
+    if gate.shape != x.shape or gate.dtype != x.dtype:
+        raise ValueError(
+            f"gate must be {tuple(x.shape)} of {x.dtype}, got {tuple(gate.shape)} of {gate.dtype}"
+        )
+    if h0 is not None and (h0.shape != x.shape[1:] or not h0.is_floating_point()):
+        raise ValueError(f"h0 must be floating point {tuple(x.shape[1:])}, got {tuple(h0.shape)} of {h0.dtype}")
+    if reset is not None and (reset.shape != x.shape[:2] or reset.dtype != torch.bool):
+        raise ValueError(f"reset must be bool {tuple(x.shape[:2])}, got {tuple(reset.shape)} of {reset.dtype}")
+    if not x.is_floating_point():
+        raise TypeError(f"x must be floating point, got {x.dtype}")
+    for name, v in (('gate', gate), ('h0', h0), ('reset', reset)):
+        if v is not None and v.device != x.device:
+            raise ValueError(f"{name} is on {v.device}, x on {x.device}")
+    from ding.ops import dispatch
+    if dispatch.use_hip_autograd(x):
+        if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise TypeError(f"x on a GPU must be float32, bfloat16 or float16, got {x.dtype}")
+        return dispatch.gated_linear_recurrence(x, gate, h0, reset)
+    return _gated_linear_recurrence_torch(x, gate, h0, reset)
+
+
+class GatedLinearRNN(nn.Module, LSTMForwardWrapper):
+    """Multi-layer gated linear recurrence with the LSTM's interface.
+
+    Layer l: [x, f] = inputs W_l^T + b_l (one library GEMM over the whole sequence), then
+    ``gated_linear_recurrence``; layers after the first add their input back. There is no product with the state, so
+    nothing but the scan runs along the time axis. The gate's bias starts at 2: a state forgets over about 8 steps.
+    ``reset`` [T, B] marks the steps that start an episode inside a sequence. The state's 'c' repeats its 'h'.
+    """
+
+    def __init__(self, input_size: int, hidden_size: int, num_layers: int = 1):
+        super().__init__()
+        self.input_size = input_size
+        self.hidden_size = hidden_size
+        self.num_layers = num_layers
+        sizes = [input_size] + [hidden_size] * (num_layers - 1)
+        self.project = nn.ModuleList([nn.Linear(size, 2 * hidden_size) for size in sizes])
+        for layer in self.project:
+            nn.init.constant_(layer.bias[hidden_size:], 2.0)
+
+    def forward(self, inputs: torch.Tensor, prev_state=None, list_next_state: bool = True,
+                reset: Optional[torch.Tensor] = None):
+        """inputs [T, B, input_size]; returns (output [T, B, H], next_state)."""
+        prev_state = self._before_forward(inputs, prev_state)
+        x, last = inputs, []
+        for i, layer in enumerate(self.project):
+            value, gate = layer(x).chunk(2, dim=-1)
+            h, state = gated_linear_recurrence(value, gate, prev_state[0][i], reset)
+            last.append(state)
+            x = h if i == 0 else x + h
+        state = torch.stack(last)
+        return x, self._after_forward((state, state), list_next_state)
+
+
 def get_lstm(
     lstm_type: str,
     input_size: int,
@@ -199,11 +294,13 @@ def get_lstm(
     seq_len: Optional[int] = None,
     batch_size: Optional[int] = None,
 ) -> nn.Module:
-    assert lstm_type in ('normal', 'pytorch', 'hpc', 'gru')
+    assert lstm_type in ('normal', 'pytorch', 'hpc', 'gru', 'glr')
     if lstm_type in ('normal', 'hpc'):
         # 'hpc' maps to the same module; its pointwise stage dispatches to the
         # HIP kernel lane on GPU once ding/ops ships the fused op.
         return LSTM(input_size, hidden_size, num_layers, norm_type, dropout)
     if lstm_type == 'pytorch':
         return PytorchLSTM(input_size, hidden_size, num_layers)
+    if lstm_type == 'glr':
+        return GatedLinearRNN(input_size, hidden_size, num_layers)
     return GRU(input_size, hidden_size, num_layers)
