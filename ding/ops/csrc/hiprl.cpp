@@ -59,6 +59,10 @@ std::vector<torch::Tensor> linrec_bwd(
     torch::Tensor x, torch::Tensor gate, torch::Tensor reset, torch::Tensor starts, torch::Tensor grad_h,
     torch::Tensor grad_last, int64_t want_h0
 );
+torch::Tensor newton_schulz(
+    torch::Tensor matrices, int64_t steps, double a, double b, double c, double eps, double scale_x, double scale_g,
+    double scale_b
+);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "DI-engine MI355X HIP kernels (gfx950)";
@@ -80,4 +84,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("token_log_prob_bwd", &token_log_prob_bwd, "gradient of token_log_prob_fwd");
     m.def("linrec_fwd", &linrec_fwd, "gated linear recurrence forward");
     m.def("linrec_bwd", &linrec_bwd, "gated linear recurrence backward");
+    m.def("newton_schulz", &newton_schulz, "orthogonalisation by Newton-Schulz products");
 }

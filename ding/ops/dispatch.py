@@ -423,3 +423,10 @@ def gated_linear_recurrence(x, gate, h0, reset):
     x = x if x.stride(-1) == 1 else x.contiguous()
     gate = gate if gate.stride(-1) == 1 else gate.contiguous()
     return _GatedLinearRecurrence.apply(x, gate, h0, None if reset is None else reset.contiguous())
+
+
+def newton_schulz(matrices, steps: int, coefficients, eps: float, scales):
+    """matrices [batch, m, n] -> the same, orthogonalised. ``scales`` are the
+    powers of two by which X, X X^T and b X X^T + c (X X^T)^2 are multiplied
+    to be held in half precision pairs."""
+    return _load().newton_schulz(matrices, steps, *coefficients, eps, *scales)

@@ -5,7 +5,7 @@ from .data_helper import (
 )
 from .optimizer_helper import (
     Adam, RMSprop, PCGrad, calculate_grad_norm, calculate_grad_norm_without_bias_two_norm, grad_ignore_norm,
-    grad_ignore_value, configure_weight_decay,
+    grad_ignore_value, configure_weight_decay, Muon, orthogonalize,
 )
 from .checkpoint_helper import build_checkpoint_helper, CheckpointHelper, auto_checkpoint, CountVar
 from .loss import LabelSmoothCELoss, SoftLogitsLoss, MultiLogitsLoss, ContrastiveLoss, build_ce_criterion

@@ -1,4 +1,5 @@
-"""Optimizers with integrated gradient clip/ignore, and PCGrad.
+"""Optimizers with integrated gradient clip/ignore, PCGrad, and the
+orthogonalised update of weight matrices (orthogonalize, Muon).
 
 Parity: reference ding/torch_utils/optimizer_helper.py (Adam:107,
 RMSprop:395, PCGrad:650, grad monitoring helpers).
@@ -9,7 +10,8 @@ Clip semantics (matching the reference's option set):
   zeroes the whole step when the threshold trips.
 """
 import math
-from typing import Iterable, List, Optional, Union
+from functools import lru_cache
+from typing import Iterable, List, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -250,6 +252,221 @@ class RMSprop(torch.optim.RMSprop):
         elif t == 'ignore_norm':
             grad_ignore_norm(params, self._ignore_value, self._ignore_norm_type)
         return super().step(closure)
+
+
+@lru_cache(maxsize=64)
+def _newton_schulz_scales(coefficients: Tuple[float, float, float], steps: int) -> Tuple[float, float, float]:
+    """Powers of two that bring X, X X^T and b X X^T + c (X X^T)^2 near the top of half precision without passing it.
+
+    No entry of a matrix is larger than its largest singular value, and those follow s -> a s + b s^3 + c s^5 from
+    [0, 1]: the largest value of that polynomial over the range so far lies at an end or where its derivative vanishes.
+    """
+    a, b, c = coefficients
+    top, most_x, most_b = 1.001, 1.001, 0.0
+    for _ in range(steps):
+        ends = [top ** 2]
+        inner = ends + ([-b / (2 * c)] if c != 0 and 0 < -b / (2 * c) < top ** 2 else [])
+        most_b = max([most_b] + [abs(b * u + c * u * u) for u in inner])
+        root = 9 * b * b - 20 * a * c
+        for sign in (-1, 1):
+            u = (-3 * b + sign * math.sqrt(max(root, 0.0))) / (10 * c) if c != 0 else (-a / (3 * b) if b else 0.0)
+            if root >= 0 and 0 < u < top ** 2:
+                ends.append(u)
+        top = 1.001 * max(abs(math.sqrt(u) * (a + b * u + c * u * u)) for u in ends)
+        if not top < 64:
+            raise ValueError(f"coefficients {coefficients} let singular values grow without bound in {steps} steps")
+        most_x = max(most_x, top)
+    return tuple(2.0 ** math.floor(math.log2(32768 / max(v, 2.0 ** -10))) for v in (most_x, most_x ** 2, most_b))
+
+
+def _orthogonalize_torch(x: torch.Tensor, steps: int, coefficients: Tuple[float, float, float], eps: float):
+    a, b, c = coefficients
+    dtype, tall = x.dtype, x.shape[-2] > x.shape[-1]
+    x = x.transpose(-2, -1) if tall else x
+    x = x.to(torch.float64 if dtype == torch.float64 else torch.float32).contiguous()
+    # the norm in 64 bits: squares of 32-bit numbers overflow and vanish
+    x = (x / (x.double().square().sum((-2, -1), keepdim=True).sqrt() + eps)).to(x.dtype)
+    for _ in range(steps):
+        gram = torch.matmul(x, x.transpose(-2, -1).contiguous())
+        x = a * x + torch.matmul(b * gram + c * torch.matmul(gram, gram), x)
+    return (x.transpose(-2, -1) if tall else x).to(dtype).contiguous()
+
+
+@torch.no_grad()
+def orthogonalize(
+        matrix: torch.Tensor,
+        steps: int = 5,
+        coefficients: Tuple[float, float, float] = (3.4445, -4.7750, 2.0315),
+        eps: float = 1e-7,
+) -> torch.Tensor:
+    """
+    Overview:
+        Moves the singular values of a matrix towards 1 and leaves its singular vectors: Newton-Schulz steps
+        ``X <- a X + (b X X^T + c (X X^T)^2) X`` from ``X = matrix / (|matrix|_F + eps)``. The default coefficients
+        bring singular values of more than about 1/300 of the norm into [0.7, 1.2] in five steps. On a GPU the
+        products run on the matrix units to 22 bits (HIP kernels, ding/ops/csrc/ortho_ops.hip). Not differentiable.
+    Arguments:
+        - matrix (:obj:`torch.Tensor`): [..., m, n] of float32, bfloat16 or float16, any strides; a batch is \
+            orthogonalised together, which is faster than one matrix after the other.
+        - steps (:obj:`int`): Number of steps, at least 1.
+        - coefficients (:obj:`Tuple[float, float, float]`): a, b and c.
+        - eps (:obj:`float`): Is added to the norm: a zero matrix gives zeros. On a GPU entries are held to about \
+            1e-11 of the normalised matrix, so one whose norm is far below ``eps`` loses its digits.
+    Returns:
+        - update (:obj:`torch.Tensor`): [..., m, n], a new dense tensor of the same type.
+    """
+    if matrix.dim() < 2 or not matrix.is_floating_point():
+        raise ValueError(f"matrix must be floating point [..., m, n], got {tuple(matrix.shape)} of {matrix.dtype}")
+    if steps < 1:
+        raise ValueError(f"steps must be at least 1, got {steps}")
+    if not eps > 0:
+        raise ValueError(f"eps must be positive, got {eps}")
+    coefficients = tuple(float(v) for v in coefficients)
+    if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
+        raise ValueError(f"coefficients must be three finite numbers, got {coefficients}")
+    scales = _newton_schulz_scales(coefficients, int(steps))
+    from ding.ops import dispatch
+    if not dispatch.use_hip_autograd(matrix):
+        return _orthogonalize_torch(matrix, steps, coefficients, eps)
+    if matrix.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"matrix on a GPU must be float32, bfloat16 or float16, got {matrix.dtype}")
+    flat = matrix.reshape(-1, *matrix.shape[-2:]) if matrix.numel() else matrix.new_empty(0, 1, 1)
+    return dispatch.newton_schulz(flat, int(steps), coefficients, float(eps), scales).view(matrix.shape)
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum whose update of a weight matrix is orthogonalised, with the same gradient clip/ignore as ``RMSprop``.
+
+    A parameter of two or more dimensions is taken as the matrix [shape[0], rest]. Its update is
+    ``orthogonalize(g + momentum * buf)`` times 0.2 sqrt(max(rows, cols)), which has the root mean square of a usual
+    Adam step, so a learning rate tuned for Adam fits. Other parameters, and groups with ``use_adam=True`` (embeddings,
+    output heads), take Adam steps with the same learning rate. Matrices of one shape are orthogonalised together.
+    Weight decay is decoupled. Momentum and Adam states are 32 bit whatever the parameter's type; nothing is read back
+    to the host, so a step can be captured into a graph unless an ``ignore_*`` clip is chosen.
+    """
+
+    def __init__(
+        self,
+        params: Iterable,
+        lr: float = 1e-3,
+        momentum: float = 0.95,
+        nesterov: bool = True,
+        weight_decay: float = 0,
+        ns_steps: int = 5,
+        ns_coefficients: Tuple[float, float, float] = (3.4445, -4.7750, 2.0315),
+        ns_eps: float = 1e-7,
+        betas: Tuple[float, float] = (0.9, 0.999),
+        eps: float = 1e-8,
+        use_adam: bool = False,
+        grad_clip_type: Optional[str] = None,
+        clip_value: Optional[float] = None,
+        clip_norm_type: float = 2.0,
+        ignore_value: Optional[float] = None,
+        ignore_norm_type: float = 2.0,
+    ):
+        if not 0 <= momentum < 1:
+            raise ValueError(f"momentum must be in [0, 1), got {momentum}")
+        if lr < 0 or weight_decay < 0:
+            raise ValueError(f"lr and weight_decay must not be negative, got {lr} and {weight_decay}")
+        if grad_clip_type not in (None, 'clip_value', 'clip_norm', 'ignore_value', 'ignore_norm'):
+            raise KeyError(f"unknown grad_clip_type {grad_clip_type}")
+        self._grad_clip_type = grad_clip_type
+        self._clip_value = clip_value
+        self._clip_norm_type = clip_norm_type
+        self._ignore_value = ignore_value
+        self._ignore_norm_type = ignore_norm_type
+        super().__init__(
+            params,
+            dict(
+                lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, ns_steps=ns_steps,
+                ns_coefficients=ns_coefficients, ns_eps=ns_eps, betas=betas, eps=eps, use_adam=use_adam
+            )
+        )
+
+    def _params(self):
+        return [p for group in self.param_groups for p in group['params']]
+
+    def _apply_clip(self):
+        t = self._grad_clip_type
+        params = self._params()
+        if t == 'clip_value':
+            nn.utils.clip_grad_value_(params, self._clip_value)
+        elif t == 'clip_norm':
+            _fe = True if (params and all(p.is_cuda for p in params)) else None
+            nn.utils.clip_grad_norm_(params, self._clip_value, self._clip_norm_type, foreach=_fe)
+        elif t == 'ignore_value':
+            grad_ignore_value(params, self._ignore_value)
+        elif t == 'ignore_norm':
+            grad_ignore_norm(params, self._ignore_value, self._ignore_norm_type)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        self._apply_clip()
+        for group in self.param_groups:
+            params = [p for p in group['params'] if p.grad is not None]
+            if not params:
+                continue
+            if group['weight_decay'] != 0:
+                torch._foreach_mul_(params, 1 - group['lr'] * group['weight_decay'])
+            alike = {}
+            for p in params:
+                matrix = p.dim() >= 2 and not group['use_adam']
+                shape = (p.shape[0], p.numel() // p.shape[0]) if matrix and p.numel() else None
+                alike.setdefault((shape, p.dtype, p.device), []).append(p)
+            for (shape, _, _), same in alike.items():
+                if shape is None:
+                    self._adam(group, same)
+                else:
+                    self._orthogonal(group, same, shape)
+        return loss
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        super().load_state_dict(state_dict)
+        # torch casts states to their parameter's type; they are taken again in the 32 bits they were kept in
+        ids = [i for group in state_dict['param_groups'] for i in group['params']]
+        for i, p in zip(ids, self._params()):
+            for key, value in state_dict['state'].get(i, {}).items():
+                self.state[p][key] = value.detach().to(device=p.device, dtype=torch.float32, copy=True)
+
+    def _orthogonal(self, group: dict, params: List[torch.Tensor], shape: Tuple[int, int]) -> None:
+        for p in params:
+            if 'momentum_buffer' not in self.state[p]:
+                self.state[p]['momentum_buffer'] = torch.zeros_like(p, dtype=torch.float32)
+        bufs = [self.state[p]['momentum_buffer'] for p in params]
+        grads = [p.grad.float() for p in params]
+        torch._foreach_mul_(bufs, group['momentum'])
+        torch._foreach_add_(bufs, grads)
+        updates = torch._foreach_add(grads, bufs, alpha=group['momentum']) if group['nesterov'] else bufs
+        # in the weights' type: the step is rounded to it when it is added to them anyway
+        stacked = torch.stack([u.reshape(shape) for u in updates]).to(params[0].dtype)
+        update = orthogonalize(stacked, group['ns_steps'], group['ns_coefficients'], group['ns_eps'])
+        step = group['lr'] * 0.2 * math.sqrt(max(shape))
+        torch._foreach_add_(params, [u.view(p.shape) for u, p in zip(update.unbind(0), params)], alpha=-step)
+
+    def _adam(self, group: dict, params: List[torch.Tensor]) -> None:
+        beta1, beta2 = group['betas']
+        for p in params:
+            state = self.state[p]
+            if 'step' not in state:
+                state['step'] = torch.zeros((), dtype=torch.float32, device=p.device)
+                state['exp_avg'] = torch.zeros_like(p, dtype=torch.float32)
+                state['exp_avg_sq'] = torch.zeros_like(p, dtype=torch.float32)
+        steps, first, second = ([self.state[p][k] for p in params] for k in ('step', 'exp_avg', 'exp_avg_sq'))
+        grads = [p.grad.float() for p in params]
+        torch._foreach_add_(steps, 1)
+        torch._foreach_lerp_(first, grads, 1 - beta1)
+        torch._foreach_mul_(second, beta2)
+        torch._foreach_addcmul_(second, grads, grads, 1 - beta2)
+        for p, n, m, v in zip(params, steps, first, second):
+            scale = group['lr'] / (1 - beta1 ** n)
+            p.sub_((scale * m / ((v / (1 - beta2 ** n)).sqrt() + group['eps'])).to(p.dtype))
+
+    def get_grad(self) -> float:
+        return calculate_grad_norm_without_bias_two_norm(_FakeModel(self._params()))
 
 
 class PCGrad:
