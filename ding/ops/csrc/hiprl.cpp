@@ -60,8 +60,8 @@ std::vector<torch::Tensor> linrec_bwd(
     torch::Tensor grad_last, int64_t want_h0
 );
 torch::Tensor newton_schulz(
-    torch::Tensor matrices, int64_t steps, double a, double b, double c, double eps, double scale_x, double scale_g,
-    double scale_b
+    torch::Tensor matrices, int64_t steps, double a, double b, double c, double eps, std::vector<double> scales,
+    int64_t span
 );
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

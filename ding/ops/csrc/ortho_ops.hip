@@ -1,32 +1,44 @@
 // Orthogonalisation of matrices by Newton-Schulz products.
 //
-//   X_0 = M / (|M|_F + eps), transposed where M is tall;  five times or so:
-//   G = X X^T,  B = b G + c G G,  X <- a X + B X
+//   X_0 = M / (|M|_F + eps), transposed where M is tall;  `steps` times:
+//   G = X X^T,  X <- (a + b G + c G G) X
 // Each step maps every singular value s to a s + b s^3 + c s^5 and leaves the singular vectors.
 //
-// Bound by the matrix units. There is no wide 32-bit matrix instruction here, and the iteration multiplies early errors by
-// a^steps (about 500), so 16-bit factors alone lose the small singular values. Every factor is therefore held as two
-// half-precision numbers, v = (hi + lo) / scale with 22 significant bits, and a product is three matrix instructions,
+// Bound by the matrix units. The iteration multiplies early errors by a^steps (about 500), so 16-bit factors alone lose
+// the small singular values, and 32-bit matrix instructions run at a tenth of the 16-bit rate. Every factor is therefore
+// held as two half-precision numbers, v = (hi + lo) / scale with 22 significant bits, and a product is three matrix
+// instructions,
 //   hi hi + hi lo + lo hi   (lo lo is below 2^-22 of the result),
 // summed in 32 bits. The scales are powers of two that the host derives from a bound of the singular values, so that
-// nothing overflows and nothing but negligible entries becomes subnormal. G and G G are symmetric: half their tiles are
-// computed and written twice.
+// nothing overflows and nothing but negligible entries becomes subnormal. A matrix given in 16 bits needs one number an
+// entry until the first step has changed it: it is scaled by a power of two and the rest of its norm goes into the
+// products' factors.
 //
-// All three products are "row times row" (C_ij = sum_k A_ik B_jk), which needs X and its transpose: both are kept.
-// Sides are padded with zeros to a multiple of kPad, so that the product kernels have no edges.
+// Two ways through the same polynomial:
+//   direct: G, G G and the product with X every step: m^2 n + m^3 + 2 m^2 n flops (symmetric results by half);
+//   gram:   with Q = a + b G + c G G, P <- Q P and G <- Q G Q, all symmetric, and X <- P X once at the end of some steps.
+// The second is cheaper where n is larger than m, but errors of G grow by a^2 a step where those of X grow by a: it is
+// taken for results that are rounded to 16 bits, over so many steps that its error stays below a fraction of that
+// rounding (five for bfloat16, three for float16).
+//
+// All products are "row times row" (C_ij = sum_k A_ik B_jk), which needs X and its transpose: both are kept. Columns are
+// padded with zeros to a multiple of a stage's depth; rows of a tile that lie behind them are memory of ours that may
+// hold anything, and reach nothing but such rows of the results.
 #include "common.h"
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
 namespace {
 
-constexpr int kPad = 128;
 constexpr int kThreads = 256;
-constexpr int kNormBlocks = 64;
+constexpr int kNormBlocks = 256;  // at most, for one matrix
+constexpr int kStage = 32;       // depth of a stage
+constexpr int kEdge = 64;        // tile side of the packing kernel
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
+typedef float float4v __attribute__((ext_vector_type(4)));
 
 __device__ inline float to_f(float v) { return v; }
 __device__ inline float to_f(__half v) { return __half2float(v); }
@@ -43,11 +55,16 @@ struct Matrix {
     int rows, cols;
 };
 
-// two planes [batch, rows, cols] of half precision
+// Two planes of half precision. A plane lies in panels of kStage columns, [batch, panel, rows, kStage], so that what a
+// tile needs of a stage is one dense piece of memory: rows at a stride of some KB would fall into few of the memory's
+// channels (products of 2048 to 16384 columns took 1.05 to 1.35 times as long).
 struct Split {
     _Float16 *hi, *lo;
     int64_t batch_stride;
-    int cols;
+    int rows;
+    __device__ inline int64_t at(int64_t batch, int r, int k) const {
+        return batch * batch_stride + ((int64_t)(k / kStage) * rows + r) * kStage + k % kStage;
+    }
 };
 
 __device__ inline void split(float v, _Float16& hi, _Float16& lo) {
@@ -55,17 +72,33 @@ __device__ inline void split(float v, _Float16& hi, _Float16& lo) {
     lo = (_Float16)(v - (float)hi);
 }
 
-// sums of squares in 64 bits, where no square of a 32-bit number overflows or vanishes
+// Sums of squares in 64 bits, where no square of a 32-bit number overflows or vanishes. A workgroup takes lines of the
+// dense direction, 16 bytes a thread where `wide` says that lines start at such an address.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_kernel(Matrix m, double* __restrict__ partial) {
+__global__ void __launch_bounds__(kThreads) norm_kernel(Matrix m, double* __restrict__ partial, int wide) {
+    constexpr int N = 16 / sizeof(T);
     const T* p = (const T*)m.base + blockIdx.y * m.batch_stride;
     double sum = 0;
-    bool flip = m.row_stride < m.col_stride;  // walk the dense direction
-    int64_t inner = flip ? m.rows : m.cols, n = (int64_t)m.rows * m.cols;
+    bool flip = m.row_stride < m.col_stride;
+    int lines = flip ? m.cols : m.rows, length = flip ? m.rows : m.cols;
     int64_t si = flip ? m.row_stride : m.col_stride, so = flip ? m.col_stride : m.row_stride;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)kNormBlocks * kThreads) {
-        double v = to_f(p[i / inner * so + i % inner * si]);
-        sum += v * v;
+    int per = wide ? N : 1, groups = (length + per - 1) / per;
+    int64_t n = (int64_t)lines * groups;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
+        int64_t line = n < (int64_t)1 << 31 ? (unsigned)i / (unsigned)groups : i / groups;
+        int at = (int)(i - line * groups) * per;
+        const T* q = p + line * so + at * si;
+        if (wide && at + N <= length) {
+            T v[N];
+            __builtin_memcpy(v, q, 16);
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum += (double)to_f(v[e]) * to_f(v[e]);
+        } else {
+            for (int e = 0; e < per && at + e < length; ++e) {
+                double v = to_f(q[e * si]);
+                sum += v * v;
+            }
+        }
     }
     __shared__ double part[kThreads / kWave];
     for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
@@ -73,71 +106,132 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(Matrix m, double* __rest
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < kThreads / kWave; ++w) sum += part[w];
-        partial[blockIdx.y * kNormBlocks + blockIdx.x] = sum;
+        partial[blockIdx.y * gridDim.x + blockIdx.x] = sum;
     }
 }
 
-// X and its transpose from M: a 64 x 64 tile a workgroup, turned in LDS
+// X and its transpose from M: a 64 x 64 tile a workgroup, turned in LDS. With `lo` planes X = M scale / (norm + eps);
+// without, X = M times the next lower power of two, exactly, and `rest` takes what is left (in [1, 2)).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) pack_kernel(
-    Matrix m, const double* __restrict__ partial, double eps, float scale, Split x, Split xt
+    Matrix m, const double* __restrict__ partial, int parts, double eps, float scale, Split x, Split xt,
+    float* __restrict__ rest
 ) {
-    __shared__ float tile[64][65];
-    __shared__ float factor_s;
+    __shared__ float tile[kEdge][kEdge + 1];
+    __shared__ double sum_s[kThreads / kWave];
     int b = blockIdx.z;
-    if (threadIdx.x < kWave) {
-        double sum = threadIdx.x < kNormBlocks ? partial[b * kNormBlocks + threadIdx.x] : 0;
-        for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
-        if (threadIdx.x == 0) factor_s = (float)(scale / (sqrt(sum) + eps));
-    }
+    double sum = threadIdx.x < parts ? partial[b * parts + threadIdx.x] : 0;
+    for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+    if (threadIdx.x % kWave == 0) sum_s[threadIdx.x / kWave] = sum;
     __syncthreads();
-    float factor = factor_s;
+    sum = sum_s[0];
+    for (int w = 1; w < kThreads / kWave; ++w) sum += sum_s[w];
+    double whole = scale / (sqrt(sum) + eps);
+    float factor = (float)whole, left = 1.f;
+    if (!x.lo) {
+        int e;
+        frexp(whole, &e);
+        // beyond the range of 32 bits the matrix is zero or not finite
+        factor = (float)ldexp(1.0, min(max(e - 1, -120), 120));
+        left = (float)(whole / factor);
+    }
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) rest[b] = left;
     const T* p = (const T*)m.base + b * m.batch_stride;
-    int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, lane = threadIdx.x % 64;
+    int i0 = blockIdx.y * kEdge, j0 = blockIdx.x * kEdge, lane = threadIdx.x % kEdge;
     bool flip = m.row_stride < m.col_stride;
-    for (int r = threadIdx.x / 64; r < 64; r += kThreads / 64) {
+#pragma unroll 4
+    for (int r = threadIdx.x / kEdge; r < kEdge; r += kThreads / kEdge) {
         int i = flip ? lane : r, j = flip ? r : lane;
         bool in = i0 + i < m.rows && j0 + j < m.cols;
         tile[i][j] = in ? to_f(p[(i0 + i) * m.row_stride + (j0 + j) * m.col_stride]) * factor : 0.f;
     }
     __syncthreads();
-    for (int r = threadIdx.x / 64; r < 64; r += kThreads / 64) {
+#pragma unroll 4
+    for (int r = threadIdx.x / kEdge; r < kEdge; r += kThreads / kEdge) {
         _Float16 hi, lo;
         split(tile[r][lane], hi, lo);
-        int64_t at = b * x.batch_stride + (int64_t)(i0 + r) * x.cols + j0 + lane;
+        int64_t at = x.at(b, i0 + r, j0 + lane);
         x.hi[at] = hi;
-        x.lo[at] = lo;
+        if (x.lo) x.lo[at] = lo;
         split(tile[lane][r], hi, lo);
-        at = b * xt.batch_stride + (int64_t)(j0 + r) * xt.cols + i0 + lane;
+        at = xt.at(b, j0 + r, i0 + lane);
         xt.hi[at] = hi;
-        xt.lo[at] = lo;
+        if (x.lo) xt.lo[at] = lo;
     }
 }
-
-enum Kind { GRAM, SQUARE, UPDATE, LAST };
 
 struct Target {
     void* base;
     int64_t batch_stride, row_stride, col_stride;
     int rows, cols;
+    int type;  // 0: float, 1: half, 2: bfloat16
 };
 
-// C = A B^T over split factors, a TILE x TILE tile a workgroup, a quarter of it a wave.
-//   GRAM:   A = B = X;      out = G, both triangles
-//   SQUARE: A = B = G;      out = b G + c C, both triangles
-//   UPDATE: A = X^T, B = b G + c G G (symmetric): C = (B X)^T; x <- a x + C^T and its transpose to out
-//   LAST:   the same, written to the caller's matrix in its type
-template <int TILE, Kind kind, typename T>
-__global__ void __launch_bounds__(kThreads) product_kernel(
-    Split a, Split bm, int depth, float alpha, float beta, float inv_scale, Split x, Split out, Target to
+// 16 bytes from global memory into LDS without a stop in registers; lane l of a wave writes to `to` + 16 l
+__device__ inline void copy_to_lds(const void* from, void* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// Tile sides, the part of a tile that a wave computes, and the stages that are held in LDS.
+template <int TILE_, int WM_, int WN_, int STAGES_>
+struct Shape {
+    static constexpr int TILE = TILE_, WM = WM_, WN = WN_, STAGES = STAGES_;
+    static constexpr int WAVES = (TILE / WM) * (TILE / WN);
+    static constexpr int THREADS = 64 * WAVES;
+    static constexpr int PLANE = TILE * kStage;              // halves of one plane of one factor's stage
+    static constexpr int SIDE = WM % 32 || WN % 32 ? 16 : 32;  // of a matrix instruction
+    // Where a row's four 16-byte pieces lie: the 16 lanes that LDS serves at once read as many different places.
+    static __device__ inline int turn(int row) { return (row >> (SIDE == 32 ? 2 : 1)) & 3; }
+};
+
+// v_mfma of SIDE x SIDE results: lane l gives row l % SIDE of a factor, DEPTH / 8 pieces of 8 along the depth over the
+// rest of l; it holds column l % SIDE of results, 4 rows at a time
+template <int SIDE> struct Mfma;
+template <> struct Mfma<32> {
+    typedef float16v Acc;
+    static constexpr int DEPTH = 16, QUADS = 4;
+    static __device__ inline Acc run(half8 a, half8 b, Acc c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ inline int row(int q, int lane) { return q * 8 + lane / 32 * 4; }
+};
+template <> struct Mfma<16> {
+    typedef float4v Acc;
+    static constexpr int DEPTH = 32, QUADS = 1;
+    static __device__ inline Acc run(half8 a, half8 b, Acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ inline int row(int q, int lane) { return lane / 16 * 4; }
+};
+
+enum Kind { SYMMETRIC, UPDATE, LAST };
+
+// What a product is multiplied by and what is added: v = alpha rest^power C + beta E + diagonal [i = j]
+struct Epilogue {
+    float alpha, beta, diagonal;
+    const float* rest;  // [batch] or null
+    int power;          // alpha takes rest^power, beta takes rest^beta_power
+    int beta_power;
+    float inv_scale;
+};
+
+// C = A B^T over split factors of PA and PB planes, a TILE x TILE tile a workgroup.
+//   SYMMETRIC: C is symmetric: tiles of the lower triangle, written twice. E = x where beta is not 0.
+//   UPDATE:    A = X^T, B symmetric: C = (B X)^T; x <- beta x + C^T, its transpose to out. x may have one plane on the
+//              way in (PA) and has two on the way out.
+//   LAST:      the same, written to the caller's matrix in its type.
+// A stage of 32 columns is copied straight into LDS while the one before it is multiplied. Within a row of a stage the
+// four 16-byte pieces change places with the row, so that eight rows read at once fall into different banks.
+template <typename P, Kind kind, int PA, int PB>
+__global__ void __launch_bounds__(P::THREADS) product_kernel(
+    Split a, Split bm, int depth, Epilogue ep, Split x, Split out, Target to
 ) {
-    constexpr int K = 32;               // depth of a stage
-    constexpr int W = TILE / 2;         // a wave's side
-    constexpr int S = W / 32;           // matrix instructions along it
-    constexpr int CHUNKS = TILE * K / 8;  // 16-byte pieces of a plane of a stage
-    __shared__ half8 sa[2][CHUNKS], sb[2][CHUNKS];
+    typedef Mfma<P::SIDE> M;
+    constexpr int TILE = P::TILE, SIDE = P::SIDE, SI = P::WM / SIDE, SJ = P::WN / SIDE;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[P::STAGES][(PA + PB) * P::PLANE];
     int bi, bj;
-    if constexpr (kind == GRAM || kind == SQUARE) {
+    if constexpr (kind == SYMMETRIC) {
         // tile number t of the lower triangle
         int t = blockIdx.x;
         bi = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
@@ -150,73 +244,160 @@ __global__ void __launch_bounds__(kThreads) product_kernel(
     }
     int64_t batch = blockIdx.z;
     int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    int wi = wave / 2 * W, wj = wave % 2 * W;
-    float16v acc[S][S];
-    for (int i = 0; i < S; ++i)
-        for (int j = 0; j < S; ++j) acc[i][j] = (float16v)(0.f);
-    const _Float16* pa[2] = {a.hi + batch * a.batch_stride, a.lo + batch * a.batch_stride};
-    const _Float16* pb[2] = {bm.hi + batch * bm.batch_stride, bm.lo + batch * bm.batch_stride};
-    for (int k0 = 0; k0 < depth; k0 += K) {
-        __syncthreads();
+    int wi = wave / (TILE / P::WN) * P::WM, wj = wave % (TILE / P::WN) * P::WN;
+    typename M::Acc acc[SI][SJ];
 #pragma unroll
-        for (int c = threadIdx.x; c < CHUNKS; c += kThreads) {
-            int row = c / 4, piece = c % 4;
-            int at = row * 4 + (piece ^ ((row >> 1) & 3));  // eight rows' pieces fall into different banks
+    for (int i = 0; i < SI; ++i)
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                sa[p][at] = *(const half8*)(pa[p] + (int64_t)(bi * TILE + row) * a.cols + k0 + piece * 8);
-                sb[p][at] = *(const half8*)(pb[p] + (int64_t)(bj * TILE + row) * bm.cols + k0 + piece * 8);
-            }
+        for (int j = 0; j < SJ; ++j) acc[i][j] = (typename M::Acc)(0.f);
+
+    // a wave copies 16 rows of a plane at a time: lane l takes piece l % 4 of row l / 4, from where it belongs
+    constexpr int GROUPS = (PA + PB) * TILE / 16, COPIES = (GROUPS + P::WAVES - 1) / P::WAVES;
+    const _Float16* from[COPIES];
+    int place[COPIES], pitch[COPIES];
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) {
+        int group = min(c * P::WAVES + wave, GROUPS - 1);  // every wave issues as many: some copy the last group again
+        int plane = group / (TILE / 16), first = group % (TILE / 16) * 16, row = first + lane / 4;
+        int piece = (lane % 4) ^ P::turn(row);
+        const Split& f = plane < PA ? a : bm;
+        from[c] = ((plane < PA ? plane : plane - PA) ? f.lo : f.hi) +
+                  f.at(batch, (plane < PA ? bi : bj) * TILE + row, piece * 8);
+        pitch[c] = f.rows;
+        place[c] = plane * P::PLANE + first * kStage;
+    }
+    auto fetch = [&](int k0, _Float16* stage) {
+#pragma unroll
+        for (int c = 0; c < COPIES; ++c)
+            copy_to_lds(from[c] + (int64_t)k0 * pitch[c], stage + place[c]);
+    };
+    struct Factors {
+        half8 a[PA][SI], b[PB][SJ];
+    };
+    auto read = [&](Factors& f, const _Float16* stage, int ks) {
+        int piece = ks * (M::DEPTH / 8) + lane / SIDE;
+        auto at = [&](int plane, int r) {
+            return *(const half8*)(stage + plane * P::PLANE + r * kStage + (piece ^ P::turn(r)) * 8);
+        };
+#pragma unroll
+        for (int p = 0; p < PA; ++p)
+#pragma unroll
+            for (int s = 0; s < SI; ++s) f.a[p][s] = at(p, wi + s * SIDE + lane % SIDE);
+#pragma unroll
+        for (int p = 0; p < PB; ++p)
+#pragma unroll
+            for (int s = 0; s < SJ; ++s) f.b[p][s] = at(PA + p, wj + s * SIDE + lane % SIDE);
+    };
+    auto multiply = [&](const Factors& f) {
+        auto all = [&](const half8(&u)[SI], const half8(&v)[SJ]) {
+#pragma unroll
+            for (int i = 0; i < SI; ++i)
+#pragma unroll
+                for (int j = 0; j < SJ; ++j) acc[i][j] = M::run(u[i], v[j], acc[i][j]);
+        };
+        if constexpr (PA == 2) all(f.a[1], f.b[0]);
+        if constexpr (PB == 2) all(f.a[0], f.b[1]);
+        all(f.a[0], f.b[0]);
+        // the next factors' reads are spread between these products
+        constexpr int READS = PA * SI + PB * SJ, PRODUCTS = SI * SJ * (PA + PB - 1);
+#pragma unroll
+        for (int i = 0; i < READS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / READS > 0 ? PRODUCTS / READS : 1, 0);
         }
-        __syncthreads();
+    };
+    // The factors of the next product are read from LDS while the present ones are multiplied. Copies of a wave arrive
+    // in the order of their issue: when only those of the S - 2 later stages are out, the next stage's are there; after
+    // the barrier everyone's are, and everyone has read the present stage, which is overwritten then.
+    constexpr int S = P::STAGES, STEPS = kStage / M::DEPTH;
+    int stages = depth / kStage, now = 0;
+    Factors even, odd;
+    auto turn_stage = [&](int k, Factors& f) {
+        if (stages - k >= S)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * COPIES) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (k + S < stages) fetch((k + S) * kStage, lds[now]);
+        now = now + 1 == S ? 0 : now + 1;
+        read(f, lds[now], 0);  // behind the last stage it reads what is there, and nobody uses it
+    };
 #pragma unroll
-        for (int ks = 0; ks < K / 16; ++ks) {
-            half8 fa[2][S], fb[2][S];
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-                int ra = wi + s * 32 + lane % 32, rb = wj + s * 32 + lane % 32, piece = ks * 2 + lane / 32;
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    fa[p][s] = sa[p][ra * 4 + (piece ^ ((ra >> 1) & 3))];
-                    fb[p][s] = sb[p][rb * 4 + (piece ^ ((rb >> 1) & 3))];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < S; ++i)
-#pragma unroll
-                for (int j = 0; j < S; ++j) {
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[1][i], fb[0][j], acc[i][j], 0, 0, 0);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[1][j], acc[i][j], 0, 0, 0);
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[0][i], fb[0][j], acc[i][j], 0, 0, 0);
-                }
+    for (int k = 0; k < S; ++k)
+        if (k < stages) fetch(k * kStage, lds[k]);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    read(even, lds[0], 0);
+    if constexpr (STEPS == 2) {
+        for (int k = 0; k < stages; ++k) {
+            read(odd, lds[now], 1);
+            multiply(even);
+            turn_stage(k, even);
+            multiply(odd);
+        }
+    } else if constexpr (P::TILE == 192) {
+        // two sets of factors do not fit in registers beside the sums
+        for (int k = 0; k < stages; ++k) {
+            multiply(even);
+            turn_stage(k, even);
+        }
+    } else {
+        for (int k = 0; k < stages; k += 2) {
+            turn_stage(k, odd);
+            multiply(even);
+            if (k + 1 == stages) break;
+            turn_stage(k + 1, even);
+            multiply(odd);
         }
     }
-    // a lane holds column lane % 32 of rows 8 q + 4 (lane / 32) + 0..3
+
+    float alpha = ep.alpha, beta = ep.beta;
+    if (ep.rest) {
+        float r = ep.rest[batch];
+        for (int p = 0; p < ep.power; ++p) alpha *= r;
+        for (int p = 0; p < ep.beta_power; ++p) beta *= r;
+    }
 #pragma unroll
-    for (int i = 0; i < S; ++i)
+    for (int i = 0; i < SI; ++i)
 #pragma unroll
-        for (int j = 0; j < S; ++j)
+        for (int j = 0; j < SJ; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                int r = bi * TILE + wi + i * 32 + q * 8 + lane / 32 * 4, c = bj * TILE + wj + j * 32 + lane % 32;
+            for (int q = 0; q < M::QUADS; ++q) {
+                int r = bi * TILE + wi + i * SIDE + M::row(q, lane), c = bj * TILE + wj + j * SIDE + lane % SIDE;
                 half4 hi, lo;
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = acc[i][j][q * 4 + e] * alpha;
-                if constexpr (kind != GRAM) {
-                    // the element itself: of G at (c, r), of x at (c, r)
-                    int64_t at = batch * x.batch_stride + (int64_t)c * x.cols + r;
-                    half4 xh = *(const half4*)(x.hi + at), xl = *(const half4*)(x.lo + at);
+                if (beta != 0.f) {
+                    // the element itself: of a symmetric E, or of x, at (c, r)
+                    int64_t at = x.at(batch, c, r);
+                    half4 xh = *(const half4*)(x.hi + at);
+                    if constexpr (kind == SYMMETRIC || PA == 2) {
+                        half4 xl = *(const half4*)(x.lo + at);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] += beta * ((float)xh[e] + (float)xl[e]);
+                        for (int e = 0; e < 4; ++e) v[e] += beta * ((float)xh[e] + (float)xl[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] += beta * (float)xh[e];
+                    }
+                }
+                if constexpr (kind == SYMMETRIC) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (r + e == c) v[e] += ep.diagonal;
                 }
                 if constexpr (kind == LAST) {
                     if (c < to.rows)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (r + e < to.cols)
-                                ((T*)to.base)[batch * to.batch_stride + c * to.row_stride + (r + e) * to.col_stride] =
-                                    from_f<T>(v[e] * inv_scale);
+                            if (r + e < to.cols) {
+                                int64_t at = batch * to.batch_stride + c * to.row_stride + (r + e) * to.col_stride;
+                                float w = v[e] * ep.inv_scale;
+                                if (to.type == 0)
+                                    ((float*)to.base)[at] = w;
+                                else if (to.type == 1)
+                                    ((__half*)to.base)[at] = from_f<__half>(w);
+                                else
+                                    ((__hip_bfloat16*)to.base)[at] = from_f<__hip_bfloat16>(w);
+                            }
                     continue;
                 }
 #pragma unroll
@@ -227,17 +408,17 @@ __global__ void __launch_bounds__(kThreads) product_kernel(
                     lo[e] = l;
                 }
                 if constexpr (kind == UPDATE) {
-                    int64_t at = batch * x.batch_stride + (int64_t)c * x.cols + r;
+                    int64_t at = x.at(batch, c, r);
                     *(half4*)(x.hi + at) = hi;
                     *(half4*)(x.lo + at) = lo;
                 } else if (bi != bj) {
-                    int64_t at = batch * out.batch_stride + (int64_t)c * out.cols + r;
+                    int64_t at = out.at(batch, c, r);
                     *(half4*)(out.hi + at) = hi;
                     *(half4*)(out.lo + at) = lo;
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    int64_t at = batch * out.batch_stride + (int64_t)(r + e) * out.cols + c;
+                    int64_t at = out.at(batch, r + e, c);
                     out.hi[at] = hi[e];
                     out.lo[at] = lo[e];
                 }
@@ -254,12 +435,55 @@ void by_type(const torch::Tensor& x, F&& f) {
     }
 }
 
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+int64_t tiles_of(int64_t m, int64_t n, int64_t batch, bool lower, int64_t side) {
+    int64_t r = up(m, side) / side, c = up(n, side) / side;
+    return (lower ? r * (r + 1) / 2 : r * c) * batch;
+}
+
+// The tile side for the results of m x n (of which the lower triangle, or all): the one whose busiest compute unit is
+// done first. Clocks of a stage of two planes, measured: of a tile that has its compute unit to itself, and of one among
+// those that share it. Small tiles fill the chip where there are few; large ones need less from memory a product.
+int side_of(int64_t m, int64_t n, int64_t batch, bool lower) {
+    static const struct { int side; double alone, shared; } costs[] = {
+        {256, 5650, 5650}, {192, 4200, 4200}, {128, 2260, 1730}, {96, 1650, 1190}, {64, 900, 640}
+    };
+    int best = 0;
+    double least = 0;
+    for (const auto& k : costs) {
+        int64_t each = (tiles_of(m, n, batch, lower, k.side) + 255) / 256;
+        double time = std::max(k.alone, each * k.shared);
+        if (!best || time < least) {
+            least = time;
+            best = k.side;
+        }
+    }
+    return best;
+}
+
+template <typename F>
+void by_side(int side, int64_t tiles, F&& f) {
+    switch (side) {
+        case 256: f(Shape<256, 128, 64, 2>{}); break;
+        case 192: f(Shape<192, 96, 48, 3>{}); break;
+        case 128:
+            // one tile a compute unit: eight waves hide each other's waiting; else two tiles do
+            tiles <= 256 ? f(Shape<128, 64, 32, 4>{}) : f(Shape<128, 64, 64, 2>{});
+            break;
+        case 96: f(Shape<96, 48, 48, 3>{}); break;
+        default: f(Shape<64, 32, 32, 3>{}); break;
+    }
+}
+
 }  // namespace
 
-// matrices [batch, rows, cols]; the scales are powers of two with |entry| * scale < 65504
+// matrices [batch, rows, cols]. The scales are powers of two with |entry| * scale < 65504 for X, G, b G + c G G,
+// Q = a + b G + c G G, and a product of `span` Qs; `span` 0 asks for the direct way, else P is applied every `span`
+// steps.
 torch::Tensor newton_schulz(
-    torch::Tensor matrices, int64_t steps, double a, double b, double c, double eps, double scale_x, double scale_g,
-    double scale_b
+    torch::Tensor matrices, int64_t steps, double a, double b, double c, double eps, std::vector<double> scales,
+    int64_t span
 ) {
     TORCH_CHECK(matrices.is_cuda() && matrices.dim() == 3, "orthogonalize: matrices must be [batch, m, n] on a HIP device");
     c10::OptionalDeviceGuard guard(matrices.device());
@@ -268,49 +492,113 @@ torch::Tensor newton_schulz(
     int64_t batch = matrices.size(0), rows = matrices.size(1), cols = matrices.size(2);
     bool tall = rows > cols;
     int64_t m = tall ? cols : rows, n = tall ? rows : cols;
-    TORCH_CHECK(steps >= 1 && batch < 65536 && n <= (1 << 20), "orthogonalize: at least one step, fewer than 65536 "
-                "matrices and sides of up to 2^20");
-    int64_t mp = (m + kPad - 1) / kPad * kPad, np = (n + kPad - 1) / kPad * kPad;
+    TORCH_CHECK(steps >= 1 && batch < 65536 && n <= (1 << 20) && scales.size() == 5,
+                "orthogonalize: at least one step, fewer than 65536 matrices and sides of up to 2^20");
+    double sx = scales[0], sg = scales[1], sb = scales[2], sq = scales[3], sp = scales[4];
+    int lower = side_of(m, m, batch, true), rect = side_of(m, n, batch, false);
+    // rows that tiles of either side reach, and whole tiles of the packing kernel
+    int64_t mp = std::max({up(m, lower), up(m, rect), up(m, kEdge)}), np = std::max(up(n, rect), up(n, kEdge));
+    int depth_m = (int)up(m, kStage), depth_n = (int)up(n, kStage);
     Matrix in{matrices.data_ptr(), matrices.stride(0), matrices.stride(tall ? 2 : 1), matrices.stride(tall ? 1 : 2),
               (int)m, (int)n};
+    int type = matrices.scalar_type() == torch::kFloat32 ? 0 : matrices.scalar_type() == torch::kFloat16 ? 1 : 2;
     Target to{result.data_ptr(), result.stride(0), result.stride(tall ? 2 : 1), result.stride(tall ? 1 : 2), (int)m,
-              (int)n};
+              (int)n, type};
     auto half = matrices.options().dtype(torch::kFloat16);
-    auto partial = torch::empty({batch * kNormBlocks}, matrices.options().dtype(torch::kFloat64));
+    int parts = (int)std::min<int64_t>(kNormBlocks, std::max<int64_t>(1, m * n / (kThreads * 16)));
+    auto partial = torch::empty({batch * parts}, matrices.options().dtype(torch::kFloat64));
+    auto rest = torch::empty({batch}, matrices.options().dtype(torch::kFloat32));
     std::vector<torch::Tensor> kept;
     auto planes = [&](int64_t r, int64_t q) {
         kept.push_back(torch::empty({2, batch, r, q}, half));
         _Float16* p = (_Float16*)kept.back().data_ptr();
-        return Split{p, p + batch * r * q, r * q, (int)q};
+        return Split{p, p + batch * r * q, r * q, (int)r};
     };
-    Split x = planes(mp, np), xt[2] = {planes(np, mp), planes(np, mp)}, g = planes(mp, mp), bg = planes(mp, mp);
+    bool one = type != 0;  // X has one plane until it is updated
+    Split x = planes(mp, np), xt = planes(np, mp), g = planes(mp, mp), q = planes(mp, mp);
     hipStream_t stream = ding_current_stream();
     by_type(matrices, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
-        norm_kernel<T><<<dim3(kNormBlocks, (unsigned)batch), kThreads, 0, stream>>>(in, partial.data_ptr<double>());
+        int64_t dense = std::min(in.row_stride, in.col_stride), line = std::max(in.row_stride, in.col_stride);
+        int wide = dense == 1 && (line * sizeof(T)) % 16 == 0 && (in.batch_stride * sizeof(T)) % 16 == 0 &&
+                   (uintptr_t)in.base % 16 == 0;
+        norm_kernel<T><<<dim3(parts, (unsigned)batch), kThreads, 0, stream>>>(in, partial.data_ptr<double>(), wide);
         HIP_CHECK_LAST();
-        pack_kernel<T><<<dim3((unsigned)(np / 64), (unsigned)(mp / 64), (unsigned)batch), kThreads, 0, stream>>>(
-            in, partial.data_ptr<double>(), eps, (float)scale_x, x, xt[0]);
+        Split px = x, pt = xt;
+        if (one) px.lo = pt.lo = nullptr;
+        dim3 grid((unsigned)(up(n, kEdge) / kEdge), (unsigned)(up(m, kEdge) / kEdge), (unsigned)batch);
+        pack_kernel<T><<<grid, kThreads, 0, stream>>>(in, partial.data_ptr<double>(), parts, eps, (float)sx, px, pt,
+                                                      rest.data_ptr<float>());
         HIP_CHECK_LAST();
-        constexpr int TILE = 128;
-        unsigned tiles = (unsigned)(mp / TILE), wide = (unsigned)(np / TILE);
-        dim3 half_grid(tiles * (tiles + 1) / 2, 1, (unsigned)batch), grid(wide, tiles, (unsigned)batch);
-        for (int64_t s = 0; s < steps; ++s) {
-            Split from = xt[s % 2], next = xt[(s + 1) % 2];
-            product_kernel<TILE, GRAM, T><<<half_grid, kThreads, 0, stream>>>(
-                x, x, (int)np, (float)(scale_g / (scale_x * scale_x)), 0.f, 0.f, x, g, to);
-            product_kernel<TILE, SQUARE, T><<<half_grid, kThreads, 0, stream>>>(
-                g, g, (int)mp, (float)(c * scale_b / (scale_g * scale_g)), (float)(b * scale_b / scale_g), 0.f, g, bg,
-                to);
-            float alpha = (float)(1.0 / scale_b);
-            if (s + 1 < steps)
-                product_kernel<TILE, UPDATE, T><<<grid, kThreads, 0, stream>>>(
-                    from, bg, (int)mp, alpha, (float)a, 0.f, x, next, to);
-            else
-                product_kernel<TILE, LAST, T><<<grid, kThreads, 0, stream>>>(
-                    from, bg, (int)mp, alpha, (float)a, (float)(1.0 / scale_x), x, next, to);
-            HIP_CHECK_LAST();
-        }
     });
+    // out = (alpha A B^T + beta E) scaled, for symmetric results
+    auto symmetric = [&](Split u, Split v, int depth, Epilogue ep, Split e, Split out, bool single) {
+        by_side(lower, tiles_of(m, m, batch, true, lower), [&](auto shape) {
+            using P = decltype(shape);
+            unsigned r = (unsigned)up(m, P::TILE) / P::TILE;
+            dim3 grid(r * (r + 1) / 2, 1, (unsigned)batch);
+            if (single)
+                product_kernel<P, SYMMETRIC, 1, 1><<<grid, P::THREADS, 0, stream>>>(u, v, depth, ep, e, out, to);
+            else
+                product_kernel<P, SYMMETRIC, 2, 2><<<grid, P::THREADS, 0, stream>>>(u, v, depth, ep, e, out, to);
+        });
+        HIP_CHECK_LAST();
+    };
+    // x <- beta x + p x
+    auto update = [&](Split p, double scale, double beta, bool last, Split& next) {
+        Epilogue ep{(float)(1.0 / scale), (float)beta, 0.f, one ? rest.data_ptr<float>() : nullptr, 1, 1,
+                    (float)(1.0 / sx)};
+        by_side(rect, tiles_of(m, n, batch, false, rect), [&](auto shape) {
+            using P = decltype(shape);
+            dim3 grid((unsigned)up(n, P::TILE) / P::TILE, (unsigned)up(m, P::TILE) / P::TILE, (unsigned)batch);
+            auto go = [&](auto kernel) {
+                kernel<<<grid, P::THREADS, 0, stream>>>(xt, p, depth_m, ep, x, next, to);
+            };
+            if (last)
+                one ? go(product_kernel<P, LAST, 1, 2>) : go(product_kernel<P, LAST, 2, 2>);
+            else
+                one ? go(product_kernel<P, UPDATE, 1, 2>) : go(product_kernel<P, UPDATE, 2, 2>);
+        });
+        HIP_CHECK_LAST();
+        if (!last) std::swap(xt, next);
+        one = false;
+    };
+    auto gram = [&] {
+        symmetric(x, x, depth_n, {(float)(sg / (sx * sx)), 0.f, 0.f, one ? rest.data_ptr<float>() : nullptr, 2, 0, 0.f},
+                  x, g, one);
+    };
+    if (span == 0) {
+        Split next = steps > 1 ? planes(np, mp) : xt;
+        for (int64_t s = 0; s < steps; ++s) {
+            gram();
+            symmetric(g, g, depth_m, {(float)(c * sb / (sg * sg)), (float)(b * sb / sg), 0.f, nullptr, 0, 0, 0.f}, g, q,
+                      false);
+            update(q, sb, a, s + 1 == steps, next);
+        }
+        return result;
+    }
+    Split next = steps > span ? planes(np, mp) : xt;
+    Split p[2] = {planes(mp, mp), planes(mp, mp)}, y = planes(mp, mp);
+    for (int64_t s = 0; s < steps; s += span) {
+        int64_t count = std::min(span, steps - s);
+        gram();
+        for (int64_t i = 0; i < count; ++i) {
+            // P is Q of the first step; it is written in P's scale then
+            Split into = i == 0 ? p[0] : q;
+            double s_into = i == 0 ? sp : sq;
+            symmetric(g, g, depth_m,
+                      {(float)(c * s_into / (sg * sg)), (float)(b * s_into / sg), (float)(a * s_into), nullptr, 0, 0, 0.f},
+                      g, into, false);
+            if (i > 0) {
+                symmetric(q, p[(i + 1) % 2], depth_m, {(float)(1.0 / sq), 0.f, 0.f, nullptr, 0, 0, 0.f}, g, p[i % 2],
+                          false);
+            }
+            if (i + 1 < count) {
+                symmetric(into, g, depth_m, {(float)(1.0 / s_into), 0.f, 0.f, nullptr, 0, 0, 0.f}, g, y, false);
+                symmetric(y, into, depth_m, {(float)(1.0 / s_into), 0.f, 0.f, nullptr, 0, 0, 0.f}, g, g, false);
+            }
+        }
+        update(p[(count + 1) % 2], sp, 0.0, s + count == steps, next);
+    }
     return result;
 }

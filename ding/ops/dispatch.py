@@ -425,8 +425,10 @@ def gated_linear_recurrence(x, gate, h0, reset):
     return _GatedLinearRecurrence.apply(x, gate, h0, None if reset is None else reset.contiguous())
 
 
-def newton_schulz(matrices, steps: int, coefficients, eps: float, scales):
+def newton_schulz(matrices, steps: int, coefficients, eps: float, scales, span: int):
     """matrices [batch, m, n] -> the same, orthogonalised. ``scales`` are the
-    powers of two by which X, X X^T and b X X^T + c (X X^T)^2 are multiplied
-    to be held in half precision pairs."""
-    return _load().newton_schulz(matrices, steps, *coefficients, eps, *scales)
+    powers of two by which X, G = X X^T, b G + c G G, Q = a + b G + c G G and
+    a product of ``span`` Qs are multiplied to be held in half precision pairs;
+    ``span`` 0 keeps the iteration on X, else it runs on G and X is multiplied
+    every ``span`` steps."""
+    return _load().newton_schulz(matrices, steps, *coefficients, eps, list(scales), span)

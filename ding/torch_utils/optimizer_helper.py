@@ -254,19 +254,26 @@ class RMSprop(torch.optim.RMSprop):
         return super().step(closure)
 
 
-@lru_cache(maxsize=64)
-def _newton_schulz_scales(coefficients: Tuple[float, float, float], steps: int) -> Tuple[float, float, float]:
-    """Powers of two that bring X, X X^T and b X X^T + c (X X^T)^2 near the top of half precision without passing it.
+@lru_cache(maxsize=256)
+def _newton_schulz_plan(coefficients: Tuple[float, float, float], steps: int, dtype: torch.dtype, m: int, n: int):
+    """How the kernels run the iteration on an m x n matrix (m <= n): the scales and the span of ``newton_schulz``.
 
-    No entry of a matrix is larger than its largest singular value, and those follow s -> a s + b s^3 + c s^5 from
-    [0, 1]: the largest value of that polynomial over the range so far lies at an end or where its derivative vanishes.
+    The scales are powers of two that bring X, G = X X^T, b G + c G G, Q = a + b G + c G G and a product of Qs near the
+    top of half precision without passing it: no entry of a matrix is larger than its largest singular value, and those
+    follow s -> s q(s^2), q(u) = a + b u + c u^2 from [0, 1]. The largest value over the range so far lies at an end or
+    where the derivative vanishes.
+
+    The span: running on G needs 3 m^2 n + (4 span - 3) m^3 flops a span, running on X 3 m^2 n + m^3 a step, but an error
+    of G grows by max(q)^2 a step. The growth is held to 2^15 for bfloat16 and 2^8 for float16, which leaves errors (of
+    2^-22 a product, most of which cancel) a tenth of the result's rounding; float32 has no room for it.
     """
     a, b, c = coefficients
-    top, most_x, most_b = 1.001, 1.001, 0.0
+    top, most_x, most_b, qs = 1.001, 1.001, 0.0, []
     for _ in range(steps):
         ends = [top ** 2]
         inner = ends + ([-b / (2 * c)] if c != 0 and 0 < -b / (2 * c) < top ** 2 else [])
         most_b = max([most_b] + [abs(b * u + c * u * u) for u in inner])
+        qs.append(max([abs(a)] + [abs(a + b * u + c * u * u) for u in inner]))
         root = 9 * b * b - 20 * a * c
         for sign in (-1, 1):
             u = (-3 * b + sign * math.sqrt(max(root, 0.0))) / (10 * c) if c != 0 else (-a / (3 * b) if b else 0.0)
@@ -276,7 +283,17 @@ def _newton_schulz_scales(coefficients: Tuple[float, float, float], steps: int) 
         if not top < 64:
             raise ValueError(f"coefficients {coefficients} let singular values grow without bound in {steps} steps")
         most_x = max(most_x, top)
-    return tuple(2.0 ** math.floor(math.log2(32768 / max(v, 2.0 ** -10))) for v in (most_x, most_x ** 2, most_b))
+    span, room = 0, {torch.bfloat16: 2.0 ** 15, torch.float16: 2.0 ** 8}.get(dtype, 0.0)
+    least = steps * (3 * n + m)
+    for count in range(2, steps + 1):
+        growth = max(math.prod(qs[at:at + count]) for at in range(0, steps, count))
+        counts = [min(count, steps - at) for at in range(0, steps, count)]
+        flops = sum(3 * n + (4 * k - 3) * m for k in counts)
+        if max(qs) ** (2 * (count - 1)) <= room and growth < 2.0 ** 14 and flops < least:
+            least, span = flops, count
+    most_p = max(math.prod(qs[at:at + span]) for at in range(0, steps, span)) if span else 1.0
+    bounds = (most_x, most_x ** 2, most_b, max(qs), most_p)
+    return tuple(2.0 ** math.floor(math.log2(32768 / max(v, 2.0 ** -10))) for v in bounds), span
 
 
 def _orthogonalize_torch(x: torch.Tensor, steps: int, coefficients: Tuple[float, float, float], eps: float):
@@ -324,14 +341,14 @@ def orthogonalize(
     coefficients = tuple(float(v) for v in coefficients)
     if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
         raise ValueError(f"coefficients must be three finite numbers, got {coefficients}")
-    scales = _newton_schulz_scales(coefficients, int(steps))
+    plan = _newton_schulz_plan(coefficients, int(steps), matrix.dtype, *sorted(matrix.shape[-2:]))
     from ding.ops import dispatch
     if not dispatch.use_hip_autograd(matrix):
         return _orthogonalize_torch(matrix, steps, coefficients, eps)
     if matrix.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise TypeError(f"matrix on a GPU must be float32, bfloat16 or float16, got {matrix.dtype}")
     flat = matrix.reshape(-1, *matrix.shape[-2:]) if matrix.numel() else matrix.new_empty(0, 1, 1)
-    return dispatch.newton_schulz(flat, int(steps), coefficients, float(eps), scales).view(matrix.shape)
+    return dispatch.newton_schulz(flat, int(steps), coefficients, float(eps), *plan).view(matrix.shape)
 
 
 class Muon(torch.optim.Optimizer):
