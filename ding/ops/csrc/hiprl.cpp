@@ -56,8 +56,8 @@ torch::Tensor token_log_prob_bwd(
 );
 std::vector<torch::Tensor> linrec_fwd(torch::Tensor x, torch::Tensor gate, torch::Tensor h0, torch::Tensor reset);
 std::vector<torch::Tensor> linrec_bwd(
-    torch::Tensor x, torch::Tensor gate, torch::Tensor reset, torch::Tensor starts, torch::Tensor grad_h,
-    torch::Tensor grad_last, int64_t want_h0
+    torch::Tensor x, torch::Tensor gate, torch::Tensor h0, torch::Tensor reset, torch::Tensor starts,
+    torch::Tensor grad_h, torch::Tensor grad_last, int64_t want_h0
 );
 torch::Tensor newton_schulz(
     torch::Tensor matrices, int64_t steps, double a, double b, double c, double eps, std::vector<double> scales,

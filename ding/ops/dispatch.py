@@ -399,7 +399,7 @@ class _GatedLinearRecurrence(torch.autograd.Function):
         start = none if h0 is None else h0.float().contiguous()
         mask = none if reset is None else reset
         h, last, starts = _load().linrec_fwd(x, gate, start, mask)
-        ctx.save_for_backward(x, gate, mask, starts)
+        ctx.save_for_backward(x, gate, start, mask, starts)
         ctx.h0_dtype = None if h0 is None else h0.dtype
         ctx.set_materialize_grads(False)
         return h, last
@@ -407,11 +407,11 @@ class _GatedLinearRecurrence(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_h, g_last):
-        x, gate, mask, starts = ctx.saved_tensors
+        x, gate, start, mask, starts = ctx.saved_tensors
         none = x.new_empty(0)
         want_h0 = ctx.h0_dtype is not None and ctx.needs_input_grad[2]
         dx, dgate, dh0 = _load().linrec_bwd(
-            x, gate, mask, starts, none if g_h is None else g_h.contiguous(),
+            x, gate, start, mask, starts, none if g_h is None else g_h.contiguous(),
             none if g_last is None else g_last.contiguous(), int(want_h0)
         )
         return dx, dgate, dh0.to(ctx.h0_dtype) if want_h0 else None, None
