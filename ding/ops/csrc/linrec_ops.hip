@@ -14,13 +14,16 @@
 // make of a state s, A s + B. The waves' pairs are joined in LDS; the state that enters the tile comes from the tile
 // before it. Inputs are so read once, at any length.
 //
-// Tiles of one column group follow each other by a chain: a tile leaves the state after it in memory, one 64-bit word a
-// column with the value and a mark that it is there, and the next tile's first wave waits for the word. Tiles are handed
-// out by a counter, in the order of time, so that what a tile waits for has been handed out before it to a workgroup
-// that runs already and that waits, if at all, for earlier ones only: every wait ends. Loads and all arithmetic but one
-// multiplication are done before the wait. The forward pass's words stay for the backward pass: they are the states at
-// the tiles' starts, and the states within a tile are computed again from them. The backward pass runs the same chain
-// from the last tile to the first, with M_t = r_t a_t (g_t + M_{t+1}) in the place of the state.
+// Tiles of one column group follow each other by a chain in memory. A tile leaves two 64-bit words a column: its pair
+// (A, B) as soon as it has it, and the state after the tile once it knows it. To know the state before it, a tile's
+// waves look at the tiles before it, one each: the nearest known state is carried through the pairs of the tiles in
+// between, one multiplication after the other, as if the state had been handed on from tile to tile; so results do not
+// depend on who came first. The eighth wave waits for a state, the others for either word: states move eight tiles at a
+// time. Tiles are handed out by a counter, in the order of time, so that what a tile waits for has been handed out
+// before it, to a workgroup that runs already and that waits, if at all, for earlier ones only: every wait ends. The
+// forward pass's words stay for the backward pass: they hold the states at the tiles' starts, and the states within a
+// tile are computed again from them. The backward pass runs the same chain from the last tile to the first, with
+// M_t = r_t a_t (g_t + M_{t+1}) in the place of the state.
 //
 // A reset makes A a negative zero: what comes before is then not multiplied but left out, also where it is not finite.
 #include "common.h"
@@ -135,40 +138,95 @@ __device__ inline float chain(float a, float b) {
 }
 
 // bit i: an episode starts at the lane's step i
-template <typename T>
-__device__ inline void resets(const uint8_t* reset, int64_t t0, int64_t steps, int n, int batch, int64_t first,
-                              int count, int dim, uint32_t* mask) {
+template <typename T, int STEPS>
+__device__ inline void resets(const uint8_t* reset, int64_t t0, int64_t steps, int batch, int64_t first, int count,
+                              int dim, uint32_t* mask) {
     int64_t b0 = (count > 0 ? first : 0) / dim, b1 = (count > 1 ? first + 1 : (count > 0 ? first : 0)) / dim;
-    bool same = __all(b0 == b1);  // a lane's two channels may belong to two batch entries
-    mask[0] = mask[1] = 0;
-    for (int i = 0; i < n && t0 + i < steps; ++i) {
-        uint32_t v = reset[(t0 + i) * batch + b0] != 0;
-        mask[0] |= v << i;
-        if (Lane<T>::N == 2) mask[1] |= (same ? v : (uint32_t)(reset[(t0 + i) * batch + b1] != 0)) << i;
-    }
+    auto marks = [&](int64_t b) {
+        uint8_t v[STEPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) v[i] = reset[min(t0 + i, steps - 1) * batch + b];
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) m |= (uint32_t)(v[i] != 0 && t0 + i < steps) << i;
+        return m;
+    };
+    mask[0] = mask[1] = marks(b0);
+    // a lane's two channels may belong to two batch entries
+    if (Lane<T>::N == 2 && !__all(b0 == b1)) mask[1] = marks(b1);
 }
 
+// A state's word has a mark above the value. A pair's has A above B; A is at most 1, or a negative zero, or NaN, and
+// never 2.0, whose bits are turned over in it: no pair is the zero that says that nothing is there.
 typedef unsigned long long Word;
-__device__ inline void leave(Word* p, float v) {
-    __hip_atomic_store(p, (Word)1 << 32 | __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+constexpr uint32_t kTurned = 0x40000000u;
+__device__ inline void leave(Word* p, Word w) {
+    __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ inline Word look(Word* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-// the wave waits until all of its lanes' words are there
+__device__ inline Word look(const Word* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline Word state_word(float s) { return (Word)1 << 32 | __float_as_uint(s); }
+__device__ inline Word pair_word(float a, float b) {
+    return (Word)(__float_as_uint(a) ^ kTurned) << 32 | __float_as_uint(b);
+}
+
+// The words of a chain: for each tile a row of states and a row of pairs.
+struct Chain {
+    Word* words;
+    int64_t columns;
+    __device__ inline Word* state(int64_t tile, int64_t c) const { return words + 2 * tile * columns + c; }
+    __device__ inline Word* pair(int64_t tile, int64_t c) const { return words + (2 * tile + 1) * columns + c; }
+};
+
 template <int N>
-__device__ inline void await(Word* p, int count, float* v) {
-    Word w[2];
-    for (;;) {
-        bool there = true;
+struct Window {
+    float a[kMostWaves][kWave * N], b[kMostWaves][kWave * N];
+    int known[kMostWaves];
+};
+
+// The state that enters `tile`, from the tiles that lie `step` (-1 or 1) times 1 to 8 away, of which `first` is the end
+// of the chain. Every wave of the workgroup calls it; all get the state.
+template <int N, bool RESET>
+__device__ inline void entering(const Chain& chain, Window<N>& window, int64_t tile, int step, int64_t end, int64_t c,
+                                int count, int wave, int lane, float* s) {
+    int64_t from = tile + (int64_t)step * (wave + 1);
+    if (step < 0 ? from >= end : from <= end) {
+        Word state[N], pair[N];
+        bool known, there;
+        for (;;) {
+            known = there = true;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                state[j] = pair[j] = (Word)1 << 32;
+                if (j < count) {
+                    state[j] = look(chain.state(from, c + j));
+                    if (wave + 1 < kMostWaves) pair[j] = look(chain.pair(from, c + j));
+                }
+                known = known && (state[j] >> 32);
+                there = there && (pair[j] >> 32);
+            }
+            known = __all(known);
+            there = __all(there) && wave + 1 < kMostWaves;
+            if (known || there) break;
+            __builtin_amdgcn_s_sleep(1);
+        }
+        if (lane == 0) window.known[wave] = known;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            w[j] = j < count ? look(p + j) : (Word)1 << 32;
-            there = there && (w[j] >> 32);
+            window.a[wave][lane * N + j] = __uint_as_float((uint32_t)(pair[j] >> 32) ^ kTurned);
+            window.b[wave][lane * N + j] = __uint_as_float((uint32_t)(known ? state[j] : pair[j]));
         }
-        if (__all(there)) break;
-        __builtin_amdgcn_s_sleep(1);
     }
+    __syncthreads();
+    int at = 0;
+    while (!window.known[at]) ++at;  // the end of the chain knows its state, as does what the eighth wave saw
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = __uint_as_float((uint32_t)w[j]);
+    for (int j = 0; j < N; ++j) {
+        s[j] = window.b[at][lane * N + j];
+        for (int v = at - 1; v >= 0; --v)
+            s[j] = carry<RESET>(window.a[v][lane * N + j], s[j], window.b[v][lane * N + j]);
+    }
 }
 
 // the tile that this workgroup takes: column groups turn fastest, time follows
@@ -206,7 +264,7 @@ __global__ void __launch_bounds__(kMostWaves* kWave) linrec_fwd_kernel(
         rx[i] = t0 + i < steps ? rx[i] : 0;
         rf[i] = t0 + i < steps ? rf[i] : open_gate((T*)nullptr);
     }
-    if (RESET) resets<T>(reset, t0, steps, STEPS, batch, c, count, dim, mask);
+    if (RESET) resets<T, STEPS>(reset, t0, steps, batch, c, count, dim, mask);
     // the wave's steps from nothing: h_t = add[t] + keep[t] s for a state s before them
     float add[STEPS][N], keep[STEPS][N], A[N], B[N];
 #pragma unroll
@@ -223,16 +281,17 @@ __global__ void __launch_bounds__(kMostWaves* kWave) linrec_fwd_kernel(
             add[i][j] = B[j];
             keep[i][j] = A[j];
         }
-    __shared__ float la[kMostWaves][kWave * N], lb[kMostWaves][kWave * N], start[kWave * N];
+    __shared__ float la[kMostWaves][kWave * N], lb[kMostWaves][kWave * N];
+    __shared__ Window<N> window;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         la[wave][lane * N + j] = A[j];
         lb[wave][lane * N + j] = B[j];
     }
     __syncthreads();
-    float s[2];
+    Chain links{words, columns};
+    float s[2], ta[N], tb[N];
     if (wave == 0) {
-        float ta[N], tb[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             ta[j] = A[j], tb[j] = B[j];
@@ -241,29 +300,28 @@ __global__ void __launch_bounds__(kMostWaves* kWave) linrec_fwd_kernel(
                 tb[j] = carry<RESET>(wa, tb[j], lb[w][lane * N + j]);
                 ta[j] = chain<RESET>(ta[j], wa);
             }
+            if (tile > 0 && tile + 1 < tiles && j < count) leave(links.pair(tile, c + j), pair_word(ta[j], tb[j]));
         }
-        if (tile == 0) {
+    }
+    if (tile == 0) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) s[j] = h0 && j < count ? h0[c + j] : 0.f;
-        } else {
-            await<N>(words + (tile - 1) * columns + c, count, s);
-        }
+        for (int j = 0; j < N; ++j) s[j] = h0 && j < count ? h0[c + j] : 0.f;
+    } else {
+        entering<N, RESET>(links, window, tile, -1, 0, c, count, wave, lane, s);
+    }
+    if (wave == 0) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             float after = carry<RESET>(ta[j], s[j], tb[j]);
             if (j < count) {
-                if (tile + 1 < tiles) leave(words + tile * columns + c + j, after);
+                if (tile + 1 < tiles) leave(links.state(tile, c + j), state_word(after));
                 else last[c + j] = after;
             }
-            start[lane * N + j] = s[j];
         }
     }
-    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        s[j] = start[lane * N + j];
+    for (int j = 0; j < N; ++j)
         for (int w = 0; w < wave; ++w) s[j] = carry<RESET>(la[w][lane * N + j], s[j], lb[w][lane * N + j]);
-    }
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
         float v[2];
@@ -274,7 +332,7 @@ __global__ void __launch_bounds__(kMostWaves* kWave) linrec_fwd_kernel(
 }
 
 template <typename T, int STEPS, bool RESET>
-__global__ void __launch_bounds__(kMostWaves* kWave) linrec_bwd_kernel(
+__global__ void __launch_bounds__(kMostWaves* kWave, 4) linrec_bwd_kernel(
     Seq x, Seq f, const float* __restrict__ h0, const uint8_t* __restrict__ reset, const Word* __restrict__ starts,
     const T* __restrict__ g, const float* __restrict__ g_last, T* __restrict__ dx, T* __restrict__ df,
     float* __restrict__ dh0, Word* __restrict__ words, unsigned* __restrict__ counter, int64_t steps, int batch,
@@ -314,7 +372,7 @@ __global__ void __launch_bounds__(kMostWaves* kWave) linrec_bwd_kernel(
             for (int j = 0; j < N; ++j) e[i][j] = odds(value_of(rf[i], j, (T*)nullptr));
         }
     }
-    if (RESET) resets<T>(reset, t0, steps, STEPS, batch, c, count, dim, mask);
+    if (RESET) resets<T, STEPS>(reset, t0, steps, batch, c, count, dim, mask);
     // a state s before the wave's steps becomes A s + B after them; M after them becomes A M + Q before them
     float A[N], B[N], Q[N];
 #pragma unroll
@@ -331,23 +389,22 @@ __global__ void __launch_bounds__(kMostWaves* kWave) linrec_bwd_kernel(
             Q[j] = carry<RESET>(A[j], value_of(rg[i], j, (T*)nullptr), Q[j]);
         }
     __shared__ float la[kMostWaves][kWave * N], lb[kMostWaves][kWave * N], lq[kMostWaves][kWave * N];
-    __shared__ float end[kWave * N];
+    __shared__ Window<N> window;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         la[wave][lane * N + j] = A[j];
         lb[wave][lane * N + j] = B[j];
         lq[wave][lane * N + j] = Q[j];
     }
-    float s[2], m[2];
+    Chain kept{(Word*)starts, columns}, links{words, columns};
+    float s[2], m[2], ta[N], tq[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         s[j] = 0.f;
-        if (j < count)
-            s[j] = tile > 0 ? __uint_as_float((uint32_t)starts[(tile - 1) * columns + c + j]) : h0 ? h0[c + j] : 0.f;
+        if (j < count) s[j] = tile > 0 ? __uint_as_float((uint32_t)*kept.state(tile - 1, c + j)) : h0 ? h0[c + j] : 0.f;
     }
     __syncthreads();
     if (wave == 0) {
-        float ta[N], tq[N];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             ta[j] = A[j], tq[j] = Q[j];
@@ -355,50 +412,54 @@ __global__ void __launch_bounds__(kMostWaves* kWave) linrec_bwd_kernel(
                 tq[j] = carry<RESET>(ta[j], lq[w][lane * N + j], tq[j]);
                 ta[j] = chain<RESET>(ta[j], la[w][lane * N + j]);
             }
+            if (tile > 0 && tile + 1 < tiles && j < count) leave(links.pair(tile, c + j), pair_word(ta[j], tq[j]));
         }
-        if (tile == tiles - 1) {
+    }
+    if (tile == tiles - 1) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) m[j] = g_last && j < count ? g_last[c + j] : 0.f;
-        } else {
-            await<N>(words + (tile + 1) * columns + c, count, m);
-        }
+        for (int j = 0; j < N; ++j) m[j] = g_last && j < count ? g_last[c + j] : 0.f;
+    } else {
+        entering<N, RESET>(links, window, tile, 1, tiles - 1, c, count, wave, lane, m);
+    }
+    if (wave == 0) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             float before = carry<RESET>(ta[j], m[j], tq[j]);
             if (j < count) {
-                if (tile > 0) leave(words + tile * columns + c + j, before);
+                if (tile > 0) leave(links.state(tile, c + j), state_word(before));
                 else if (dh0) dh0[c + j] = before;
             }
-            end[lane * N + j] = m[j];
         }
     }
-    __syncthreads();
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         for (int w = 0; w < wave; ++w) s[j] = carry<RESET>(la[w][lane * N + j], s[j], lb[w][lane * N + j]);
-        m[j] = end[lane * N + j];
         for (int w = waves - 1; w > wave; --w) m[j] = carry<RESET>(la[w][lane * N + j], m[j], lq[w][lane * N + j]);
     }
-    float before[STEPS][N];
+    float apart[STEPS][N];  // the state before a step less the step's input
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             float a, b;
+            // the compiler would keep the gates of the first pass, for which there are no registers
+            asm volatile("" : "+v"(e[i][j]));
             gate(e[i][j], a, b);
             if (RESET && (mask[j] >> i & 1)) s[j] = 0.f;
-            before[i][j] = s[j];
-            s[j] = fmaf(a, s[j], b * value_of(rx[i], j, (T*)nullptr));
+            float in = value_of(rx[i], j, (T*)nullptr);
+            apart[i][j] = s[j] - in;
+            s[j] = fmaf(a, s[j], b * in);
         }
 #pragma unroll
     for (int i = STEPS - 1; i >= 0; --i) {
         float vx[2], vf[2];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
+            asm volatile("" : "+v"(e[i][j]));
             float a, b, G = m[j] + value_of(rg[i], j, (T*)nullptr);
             gate(e[i][j], a, b);
             vx[j] = b * G;
-            vf[j] = G * (before[i][j] - value_of(rx[i], j, (T*)nullptr)) * a * b;
+            vf[j] = G * apart[i][j] * a * b;
             m[j] = RESET && (mask[j] >> i & 1) ? 0.f : a * G;
         }
         int here = t0 + i < steps ? count : 0;
@@ -452,10 +513,10 @@ Cut cut_of(const torch::Tensor& x) {
     return cut;
 }
 
-// the chain's words, a column each for every tile, and the counter behind them, all zero
+// the chain's words, two a column for every tile, and the counter behind them, all zero
 torch::Tensor words_of(const torch::Tensor& x, const Cut& cut) {
     auto opt = x.options().dtype(torch::kInt64);
-    return cut.tiles > 1 ? torch::zeros({cut.tiles * cut.columns + 1}, opt) : torch::empty({0}, opt);
+    return cut.tiles > 1 ? torch::zeros({2 * cut.tiles * cut.columns + 1}, opt) : torch::empty({0}, opt);
 }
 
 template <typename F>
@@ -489,7 +550,7 @@ std::vector<torch::Tensor> linrec_fwd(torch::Tensor x, torch::Tensor gate, torch
         linrec_fwd_kernel<T, decltype(n)::value, decltype(cuts)::value>
             <<<(unsigned)(cut.groups * cut.tiles), cut.waves * kWave, 0, ding_current_stream()>>>(
                 seq_of(x), seq_of(gate), h0p, rp, (T*)h.data_ptr(), last.data_ptr<float>(), w,
-                w ? (unsigned*)(w + cut.tiles * cut.columns) : nullptr, x.size(0), (int)x.size(1), (int)x.size(2),
+                w ? (unsigned*)(w + 2 * cut.tiles * cut.columns) : nullptr, x.size(0), (int)x.size(1), (int)x.size(2),
                 cut.groups, cut.tiles);
     });
     HIP_CHECK_LAST();
@@ -523,7 +584,7 @@ std::vector<torch::Tensor> linrec_bwd(
         linrec_bwd_kernel<T, decltype(n)::value, decltype(cuts)::value>
             <<<(unsigned)(cut.groups * cut.tiles), cut.waves * kWave, 0, ding_current_stream()>>>(
                 seq_of(x), seq_of(gate), h0p, rp, sp, (const T*)gp, lp, (T*)dx.data_ptr(), (T*)df.data_ptr(),
-                want_h0 ? dh0.data_ptr<float>() : nullptr, w, w ? (unsigned*)(w + cut.tiles * cut.columns) : nullptr,
+                want_h0 ? dh0.data_ptr<float>() : nullptr, w, w ? (unsigned*)(w + 2 * cut.tiles * cut.columns) : nullptr,
                 steps, (int)x.size(1), (int)x.size(2), cut.groups, cut.tiles);
     });
     HIP_CHECK_LAST();
