@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <c10/hip/HIPStream.h>
 
 // current PyTorch stream for this device (hipStream_t)
@@ -22,3 +23,16 @@ static inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
         hipError_t e = hipGetLastError();                                                \
         TORCH_CHECK(e == hipSuccess, "HIP kernel launch failed: ", hipGetErrorString(e)); \
     } while (0)
+
+// What an operator's backward pass returns: where gradients of gradients are asked for they are refused, not taken for
+// zero.
+static inline torch::autograd::variable_list ding_once_differentiable(
+    torch::autograd::variable_list grads, const char* name
+) {
+    if (!at::GradMode::is_enabled()) return grads;
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        std::string("trying to differentiate twice a function that is differentiable once: ") + name,
+        (int64_t)grads.size()
+    );
+    return (*error)(std::move(grads));
+}

@@ -45,19 +45,12 @@ std::vector<torch::Tensor> vtrace_bwd(
     torch::Tensor t_logit, torch::Tensor row_out, torch::Tensor value, torch::Tensor ret, torch::Tensor adv,
     torch::Tensor action, torch::Tensor weight, torch::Tensor gscales
 );
-std::vector<torch::Tensor> token_log_prob_fwd(
-    torch::Tensor logits, torch::Tensor index, double temperature, int64_t ignore, int64_t has_ignore,
-    int64_t want_entropy, int64_t top
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> token_log_prob(
+    torch::Tensor logits, torch::Tensor index, double temperature, c10::optional<int64_t> ignore_index, bool entropy,
+    int64_t top_k
 );
-torch::Tensor token_log_prob_bwd(
-    torch::Tensor logits, torch::Tensor index, torch::Tensor stats, torch::Tensor entropy, torch::Tensor top_index,
-    torch::Tensor grad_log_prob, torch::Tensor grad_entropy, torch::Tensor grad_top, double temperature,
-    int64_t ignore, int64_t has_ignore
-);
-std::vector<torch::Tensor> linrec_fwd(torch::Tensor x, torch::Tensor gate, torch::Tensor h0, torch::Tensor reset);
-std::vector<torch::Tensor> linrec_bwd(
-    torch::Tensor x, torch::Tensor gate, torch::Tensor h0, torch::Tensor reset, torch::Tensor starts,
-    torch::Tensor grad_h, torch::Tensor grad_last, int64_t want_h0
+std::tuple<torch::Tensor, torch::Tensor> gated_linear_recurrence(
+    torch::Tensor x, torch::Tensor gate, c10::optional<torch::Tensor> h0, c10::optional<torch::Tensor> reset
 );
 torch::Tensor newton_schulz(
     torch::Tensor matrices, int64_t steps, double a, double b, double c, double eps, std::vector<double> scales,
@@ -80,9 +73,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("conv_wrw_nhwc", &conv_wrw_nhwc, "NHWC conv2d backward-weights (fp32, register-tiled)");
     m.def("vtrace_fwd", &vtrace_fwd, "fused v-trace loss forward");
     m.def("vtrace_bwd", &vtrace_bwd, "fused v-trace loss backward");
-    m.def("token_log_prob_fwd", &token_log_prob_fwd, "token log probabilities, entropy and top alternatives");
-    m.def("token_log_prob_bwd", &token_log_prob_bwd, "gradient of token_log_prob_fwd");
-    m.def("linrec_fwd", &linrec_fwd, "gated linear recurrence forward");
-    m.def("linrec_bwd", &linrec_bwd, "gated linear recurrence backward");
+    // these call into autograd, whose threads may need the interpreter
+    m.def("token_log_prob", &token_log_prob, "token log probabilities, entropy and top alternatives, with gradient",
+          py::call_guard<py::gil_scoped_release>());
+    m.def("gated_linear_recurrence", &gated_linear_recurrence, "gated linear recurrence, with gradient",
+          py::call_guard<py::gil_scoped_release>());
     m.def("newton_schulz", &newton_schulz, "orthogonalisation by Newton-Schulz products");
 }

@@ -478,10 +478,9 @@ void check_seq(const torch::Tensor& v, const torch::Tensor& x) {
                 "gated_linear_recurrence: T must be at least 1 and B * D below 2^31");
 }
 
-// an empty tensor stands for one that is not there
 template <typename T>
 const T* given(const torch::Tensor& v, const torch::Tensor& x, int64_t n, c10::ScalarType type) {
-    if (v.numel() == 0) return nullptr;
+    if (!v.defined() || v.numel() == 0) return nullptr;
     TORCH_CHECK(v.device() == x.device() && v.is_contiguous() && v.numel() == n && v.scalar_type() == type,
                 "gated_linear_recurrence: an argument has another size, type, layout or device");
     return (const T*)v.data_ptr();
@@ -530,8 +529,6 @@ void by_case(const torch::Tensor& x, const Cut& cut, bool reset, F&& f) {
             reset ? f(null, many, std::true_type{}) : f(null, many, std::false_type{});
     });
 }
-
-}  // namespace
 
 std::vector<torch::Tensor> linrec_fwd(torch::Tensor x, torch::Tensor gate, torch::Tensor h0, torch::Tensor reset) {
     check_seq(x, x);
@@ -589,4 +586,47 @@ std::vector<torch::Tensor> linrec_bwd(
     });
     HIP_CHECK_LAST();
     return {dx, df, dh0};
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Recurrence : torch::autograd::Function<Recurrence> {
+    static variable_list forward(AutogradContext* ctx, torch::Tensor x, torch::Tensor gate,
+                                 c10::optional<torch::Tensor> h0, c10::optional<torch::Tensor> reset) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto start = h0 ? h0->to(torch::kFloat32).contiguous() : torch::Tensor();
+        auto mask = reset ? reset->contiguous() : torch::Tensor();
+        auto out = linrec_fwd(x, gate, start, mask);
+        ctx->save_for_backward({x, gate, start, mask, out[2]});
+        ctx->saved_data["h0"] = h0 ? (int64_t)h0->scalar_type() : (int64_t)-1;
+        ctx->set_materialize_grads(false);
+        return {out[0], out[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        auto kept = ctx->get_saved_variables();
+        int64_t type = ctx->saved_data["h0"].toInt();
+        bool want = type >= 0 && ctx->needs_input_grad(2);
+        variable_list out;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            auto dense = [](const torch::Tensor& t) { return t.defined() ? t.contiguous() : t; };
+            out = linrec_bwd(kept[0], kept[1], kept[2], kept[3], kept[4], dense(g[0]), dense(g[1]), want);
+            if (want) out[2] = out[2].to((c10::ScalarType)type);
+            else out[2] = torch::Tensor();
+        }
+        out.push_back(torch::Tensor());
+        return ding_once_differentiable(std::move(out), "gated_linear_recurrence");
+    }
+};
+
+}  // namespace
+
+// x, gate [T, B, D], h0 [B, D], reset [T, B] -> h, the last state; differentiable once
+std::tuple<torch::Tensor, torch::Tensor> gated_linear_recurrence(
+    torch::Tensor x, torch::Tensor gate, c10::optional<torch::Tensor> h0, c10::optional<torch::Tensor> reset
+) {
+    auto dense = [](torch::Tensor v) { return v.stride(-1) == 1 || v.size(-1) == 1 ? v : v.contiguous(); };
+    auto out = Recurrence::apply(dense(x), dense(gate), h0, reset);
+    return {out[0], out[1]};
 }

@@ -499,17 +499,33 @@ __global__ void __launch_bounds__(kThreads) token_segment_bwd(
 
 // ------------------------------------------------------------------------------------------------------------- host
 
-Rows rows_of(const torch::Tensor& logits) {
-    TORCH_CHECK(logits.is_cuda() && logits.dim() == 3 && (logits.stride(2) == 1 || logits.size(2) == 1),
-                "token_log_prob: logits must be [outer, inner, V] on a HIP device with unit stride along V");
-    return {logits.data_ptr(), logits.size(1), logits.stride(0), logits.stride(1)};
+// Leading dimensions fold into two where their strides allow it; `logits` is replaced by a dense copy where not.
+Rows rows_of(torch::Tensor& logits) {
+    for (;;) {
+        int64_t size[2] = {1, 1}, stride[2] = {0, 0};
+        int n = 0;  // folded dimensions so far, from the inner side
+        bool fits = logits.stride(-1) == 1 || logits.size(-1) == 1;
+        for (int64_t d = logits.dim() - 2; d >= 0 && fits; --d) {
+            if (logits.size(d) == 1) continue;
+            if (n > 0 && logits.stride(d) == stride[n - 1] * size[n - 1]) {
+                size[n - 1] *= logits.size(d);
+            } else if (n < 2) {
+                size[n] = logits.size(d);
+                stride[n++] = logits.stride(d);
+            } else {
+                fits = false;
+            }
+        }
+        if (fits) return {logits.data_ptr(), size[0], stride[1], stride[0]};
+        logits = logits.contiguous();
+    }
 }
 
-void check_index(const torch::Tensor& logits, const torch::Tensor& index) {
-    TORCH_CHECK(index.is_cuda() && index.device() == logits.device() && index.is_contiguous() &&
-                    index.scalar_type() == torch::kInt64 && index.numel() == logits.size(0) * logits.size(1),
-                "token_log_prob: index must be contiguous int64, one for each row, on the logits' device");
-    TORCH_CHECK(logits.size(2) >= 1 && logits.size(2) <= (1 << 30), "token_log_prob: V must be in [1, 2^30]");
+void check_args(const torch::Tensor& logits, const torch::Tensor& index) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() >= 1 && index.device() == logits.device() && index.is_contiguous() &&
+                    index.scalar_type() == torch::kInt64 && index.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+                "token_log_prob: logits [..., V] and index [...] must be on one HIP device");
+    TORCH_CHECK(logits.size(-1) >= 1 && logits.size(-1) <= (1 << 30), "token_log_prob: V must be in [1, 2^30]");
 }
 
 template <typename F>
@@ -522,26 +538,26 @@ void by_type(const torch::Tensor& x, F&& f) {
     }
 }
 
-}  // namespace
-
 std::vector<torch::Tensor> token_log_prob_fwd(
     torch::Tensor logits, torch::Tensor index, double temperature, int64_t ignore, int64_t has_ignore,
     int64_t want_entropy, int64_t top
 ) {
-    Rows rows = rows_of(logits);
-    check_index(logits, index);
+    check_args(logits, index);
     c10::OptionalDeviceGuard guard(logits.device());
+    Rows rows = rows_of(logits);
     int64_t count = index.numel();
-    int V = (int)logits.size(2);
+    int V = (int)logits.size(-1);
     int segments = cdiv(V, kSegment);
     TORCH_CHECK(top >= 0 && top <= kMostTop && top <= V, "token_log_prob: top_k must be at most ", kMostTop, " and V");
     TORCH_CHECK(top * segments <= kMostJoined, "token_log_prob: top_k of ", top, " over ", V, " entries is too much");
     auto opt = logits.options().dtype(torch::kFloat32);
-    auto log_prob = torch::empty({count}, opt);
-    auto entropy = torch::empty({want_entropy ? count : 0}, opt);
+    auto tops = index.sizes().vec();
+    tops.push_back(top);
+    auto log_prob = torch::empty(index.sizes(), opt);
+    auto entropy = want_entropy ? torch::empty(index.sizes(), opt) : torch::empty({0}, opt);
     auto stats = torch::empty({count, 2}, opt);
-    auto top_log_prob = torch::empty({count, top}, opt);
-    auto top_index = torch::empty({count, top}, opt.dtype(torch::kInt64));
+    auto top_log_prob = top ? torch::empty(tops, opt) : torch::empty({0}, opt);
+    auto top_index = top ? torch::empty(tops, opt.dtype(torch::kInt64)) : torch::empty({0}, opt.dtype(torch::kInt64));
     std::vector<torch::Tensor> result{log_prob, entropy, stats, top_log_prob, top_index};
     if (count == 0) return result;
     TORCH_CHECK(count * segments < (int64_t)1 << 31, "token_log_prob: too many rows");
@@ -597,16 +613,15 @@ torch::Tensor token_log_prob_bwd(
     torch::Tensor grad_log_prob, torch::Tensor grad_entropy, torch::Tensor grad_top, double temperature,
     int64_t ignore, int64_t has_ignore
 ) {
-    Rows rows = rows_of(logits);
-    check_index(logits, index);
+    check_args(logits, index);
     c10::OptionalDeviceGuard guard(logits.device());
+    Rows rows = rows_of(logits);
     int64_t count = index.numel();
-    int V = (int)logits.size(2);
+    int V = (int)logits.size(-1);
     int segments = cdiv(V, kSegment);
-    int top = grad_top.numel() ? (int)top_index.size(1) : 0;
-    // an empty tensor stands for a gradient that is not there
+    int top = grad_top.defined() ? (int)top_index.size(-1) : 0;
     auto given = [&](const torch::Tensor& t, int64_t n) -> const float* {
-        if (t.numel() == 0) return nullptr;
+        if (!t.defined() || t.numel() == 0) return nullptr;
         TORCH_CHECK(t.device() == logits.device() && t.is_contiguous() && t.scalar_type() == torch::kFloat32 &&
                         t.numel() == n, "token_log_prob: a gradient has another shape, type or device");
         return t.data_ptr<float>();
@@ -635,4 +650,49 @@ torch::Tensor token_log_prob_bwd(
     });
     HIP_CHECK_LAST();
     return grad;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Rows keep their maximum and log-sum (8 bytes) for the backward pass, not their probabilities.
+struct TokenLogProb : torch::autograd::Function<TokenLogProb> {
+    static variable_list forward(AutogradContext* ctx, torch::Tensor logits, torch::Tensor index, double temperature,
+                                 int64_t ignore, bool has_ignore, bool entropy, int64_t top) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto out = token_log_prob_fwd(logits, index, temperature, ignore, has_ignore, entropy, top);
+        ctx->save_for_backward({logits, index, out[2], out[1], out[4]});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["ignore"] = ignore;
+        ctx->saved_data["has_ignore"] = has_ignore;
+        ctx->set_materialize_grads(false);
+        ctx->mark_non_differentiable({out[4]});
+        return {out[0], out[1], out[3], out[4]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        auto kept = ctx->get_saved_variables();
+        torch::Tensor grad;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            auto dense = [](const torch::Tensor& t) { return t.defined() && t.numel() ? t.contiguous() : torch::Tensor(); };
+            grad = token_log_prob_bwd(kept[0], kept[1], kept[2], kept[3], kept[4], dense(g[0]), dense(g[1]), dense(g[2]),
+                                      ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore"].toInt(),
+                                      ctx->saved_data["has_ignore"].toBool());
+        }
+        torch::Tensor none;
+        return ding_once_differentiable({grad, none, none, none, none, none, none}, "token_log_prob");
+    }
+};
+
+}  // namespace
+
+// log probabilities, entropy, top log probabilities and indexes of tokens; differentiable once
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> token_log_prob(
+    torch::Tensor logits, torch::Tensor index, double temperature, c10::optional<int64_t> ignore_index, bool entropy,
+    int64_t top_k
+) {
+    index = index.to(torch::kInt64).contiguous();
+    auto out = TokenLogProb::apply(logits, index, temperature, ignore_index.value_or(0), ignore_index.has_value(),
+                                   entropy, top_k);
+    return {out[0], out[1], out[2], out[3]};
 }

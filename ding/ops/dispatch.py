@@ -340,89 +340,21 @@ def wrw_conv2d(x, weight, bias, stride):
     return _WrwConv2dFn.apply(x, weight, bias, stride)
 
 
-class _TokenLogProb(torch.autograd.Function):
-    """Token log probabilities of [outer, inner, V] logits: one pass over the
-    logits forward, one pass and one write backward. Rows keep their maximum
-    and log-sum (8 bytes) for the backward pass, not their probabilities."""
-
-    @staticmethod
-    def forward(ctx, logits, index, temperature, ignore_index, entropy, top_k):
-        ext = _load()
-        ignore = 0 if ignore_index is None else int(ignore_index)
-        log_prob, h, stats, top_log_prob, top_index = ext.token_log_prob_fwd(
-            logits, index, temperature, ignore, int(ignore_index is not None), int(entropy), top_k
-        )
-        ctx.save_for_backward(logits, index, stats, h, top_index)
-        ctx.temperature, ctx.ignore_index, ctx.ignore = temperature, ignore_index, ignore
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(top_index)
-        return log_prob, h, top_log_prob, top_index
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_log_prob, g_entropy, g_top, _):
-        logits, index, stats, h, top_index = ctx.saved_tensors
-        none = stats.new_empty(0)
-        grads = [none if g is None else g.contiguous() for g in (g_log_prob, g_entropy, g_top)]
-        grad = _load().token_log_prob_bwd(
-            logits, index, stats, h, top_index, *grads, ctx.temperature, ctx.ignore, int(ctx.ignore_index is not None)
-        )
-        return grad, None, None, None, None, None
-
-
 def token_log_prob(logits, index, temperature: float, ignore_index: Optional[int], entropy: bool, top_k: int):
     """logits [..., V], index [...] -> (log_prob, entropy or None,
-    top_log_prob or None, top_index or None), the first three in float32."""
-    shape, V = index.shape, logits.shape[-1]
-    if logits.stride(-1) != 1:
-        logits = logits.contiguous()
-    if logits.dim() < 3:
-        logits3 = logits.reshape(1, -1, V)
-    else:
-        logits3 = logits if logits.dim() == 3 else logits.flatten(0, -3)
-    args = (logits3, index.long().contiguous(), float(temperature), ignore_index, entropy, top_k)
-    log_prob, h, top_log_prob, top_index = _TokenLogProb.apply(*args)
-    return (
-        log_prob.view(shape), h.view(shape) if entropy else None,
-        top_log_prob.view(*shape, top_k) if top_k else None, top_index.view(*shape, top_k) if top_k else None
+    top_log_prob or None, top_index or None), the first three in float32 and
+    differentiable (once)."""
+    log_prob, h, top_log_prob, top_index = _load().token_log_prob(
+        logits, index, temperature, ignore_index, entropy, top_k
     )
-
-
-class _GatedLinearRecurrence(torch.autograd.Function):
-    """h_t = r_t a_t h_{t-1} + (1 - a_t) x_t over [T, B, D]. The backward pass
-    computes the states again from 32-bit starting states that the forward
-    pass keeps, so the rounded outputs are not read."""
-
-    @staticmethod
-    def forward(ctx, x, gate, h0, reset):
-        none = x.new_empty(0)
-        start = none if h0 is None else h0.float().contiguous()
-        mask = none if reset is None else reset
-        h, last, starts = _load().linrec_fwd(x, gate, start, mask)
-        ctx.save_for_backward(x, gate, start, mask, starts)
-        ctx.h0_dtype = None if h0 is None else h0.dtype
-        ctx.set_materialize_grads(False)
-        return h, last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_h, g_last):
-        x, gate, start, mask, starts = ctx.saved_tensors
-        none = x.new_empty(0)
-        want_h0 = ctx.h0_dtype is not None and ctx.needs_input_grad[2]
-        dx, dgate, dh0 = _load().linrec_bwd(
-            x, gate, start, mask, starts, none if g_h is None else g_h.contiguous(),
-            none if g_last is None else g_last.contiguous(), int(want_h0)
-        )
-        return dx, dgate, dh0.to(ctx.h0_dtype) if want_h0 else None, None
+    return log_prob, h if entropy else None, top_log_prob if top_k else None, top_index if top_k else None
 
 
 def gated_linear_recurrence(x, gate, h0, reset):
     """x, gate [T, B, D], h0 [B, D] or None, reset [T, B] bool or None ->
-    (h [T, B, D] in x's type, last state [B, D] in float32)."""
-    x = x if x.stride(-1) == 1 else x.contiguous()
-    gate = gate if gate.stride(-1) == 1 else gate.contiguous()
-    return _GatedLinearRecurrence.apply(x, gate, h0, None if reset is None else reset.contiguous())
+    (h [T, B, D] in x's type, last state [B, D] in float32), differentiable
+    (once)."""
+    return _load().gated_linear_recurrence(x, gate, h0, reset)
 
 
 def newton_schulz(matrices, steps: int, coefficients, eps: float, scales, span: int):
