@@ -9,7 +9,7 @@
 // once. Everything is kept in base 2 relative to the row's maximum: with k = log2(e) / T, d_v = (x_v - max) k,
 // s = sum 2^d, t = sum 2^d d, so log p = ln2 (d - log2 s) and H = ln2 (log2 s - t / s). All sums are 32 bit.
 //
-// A row is cut into segments of 8192 logits, one workgroup each: every thread holds 32 of them in registers, so a
+// A row is cut into equal segments of up to 8192 logits, one workgroup each: every thread holds 32 in registers, so a
 // segment is read once, also where its largest entries are wanted. The segments of a row are joined by a second,
 // small kernel; a row of one segment needs none. Rows of up to 512 entries (action sets) share a workgroup instead,
 // 16 or 64 lanes a row.
@@ -23,6 +23,7 @@ constexpr int kThreads = 256;
 constexpr int kPerThread = 32;
 constexpr int kSegment = kThreads * kPerThread;
 constexpr int kMostTop = 32;
+constexpr int64_t kManyRows = 1024;
 constexpr int kMostJoined = 4096;  // candidates that a row's segments may offer
 constexpr float kLn2 = 0.69314718055994531f;
 // 2^-200 is zero in 32 bits: entries that far below the maximum count nothing, and 0 * -inf is kept out of the sums
@@ -60,9 +61,13 @@ __device__ inline Pack<T> load_pack(const T* p) {
     __builtin_memcpy(&out, p, 16);
     return out;
 }
+// a gradient is not read again soon: it goes past the caches (2% of a forward and backward pass over 4 GB)
+typedef unsigned Quad __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 __device__ inline void store_pack(T* p, const Pack<T>& v) {
-    __builtin_memcpy(p, &v, 16);
+    Quad q;
+    __builtin_memcpy(&q, &v, 16);
+    __builtin_nontemporal_store(q, (Quad*)p);
 }
 
 // A value and its index as one integer: larger values first, among equal ones the lower index. -0 equals +0; NaN sorts
@@ -80,13 +85,27 @@ __device__ inline float value_in(unsigned long long order) {
     return __int_as_float(bits ^ ((bits >> 31) & 0x7fffffff));
 }
 
+// (x - m) k in one operation, where m k does not overflow; rows at the end of the type's range take two
+struct Distance {
+    float m, k, mk;
+    bool far;
+    __device__ inline Distance(float m_, float k_) : m(m_), k(k_), mk(m_ * k_), far(!(fabsf(m_) < 1e30f && fabsf(mk) < 1e37f)) {}
+    __device__ inline float operator()(float x) const { return far ? (x - m) * k : fmaf(x, k, -mk); }
+    template <bool FAR> __device__ inline float at(float x) const { return FAR ? (x - m) * k : fmaf(x, k, -mk); }
+    // from one reference to another, both as they are rounded
+    __device__ inline float to_reference(float other) const {
+#pragma clang fp contract(off)
+        return far ? (other - m) * k : other * k - mk;
+    }
+};
+
 struct Sums {
     float m, s, t;
 };
 
 // sums relative to `to` instead of their own maximum
 __device__ inline void shift(Sums& a, float to, float k) {
-    float d = fmaxf((a.m - to) * k, kFar);
+    float d = fmaxf(Distance(to, k).to_reference(a.m), kFar);
     float f = __builtin_amdgcn_exp2f(d);
     a.t = f * (a.t + d * a.s);
     a.s = f * a.s;
@@ -100,17 +119,30 @@ __device__ inline Sums join(Sums a, Sums b, float k) {
     return {m, a.s + b.s, a.t + b.t};
 }
 
-template <int W>
-__device__ inline float group_max(float v) {
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, W));
+// Sums and maxima over W lanes. Within 16 lanes they go through the vector unit's own lane moves, not through LDS.
+template <int CTRL>
+__device__ inline float moved(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int W, typename F>
+__device__ inline float group(float v, F&& f) {
+    v = f(v, moved<0xb1>(v));   // lanes 1 0 3 2
+    v = f(v, moved<0x4e>(v));   // lanes 2 3 0 1
+    v = f(v, moved<0x141>(v));  // the half row turned round
+    v = f(v, moved<0x140>(v));  // the row turned round
+    if constexpr (W == 64) {
+        auto row = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); };
+        v = f(f(row(0), row(16)), f(row(32), row(48)));
+    }
     return v;
 }
 template <int W>
+__device__ inline float group_max(float v) {
+    return group<W>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int W>
 __device__ inline float group_sum(float v) {
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, W);
-    return v;
+    return group<W>(v, [](float a, float b) { return a + b; });
 }
 template <int W>
 __device__ inline unsigned long long group_max(unsigned long long v) {
@@ -137,7 +169,7 @@ template <typename T>
 __device__ inline void write_row(const Out& out, int64_t r, Sums a, const T* x, int64_t token, int V, float k) {
     float log2s = log2_of(a.s);
     float lp = __builtin_nanf("");
-    if (token >= 0 && token < V) lp = ((to_f(x[token]) - a.m) * k - log2s) * kLn2;
+    if (token >= 0 && token < V) lp = (Distance(a.m, k)(to_f(x[token])) - log2s) * kLn2;
     out.log_prob[r] = lp;
     if (out.entropy) out.entropy[r] = (log2s - a.t / a.s) * kLn2;
     out.stats[2 * r] = a.m;
@@ -146,7 +178,7 @@ __device__ inline void write_row(const Out& out, int64_t r, Sums a, const T* x, 
 
 __device__ inline void write_top(const Out& out, int64_t r, int top, int j, unsigned long long order, float m,
                                  float log2s, float k) {
-    out.top_log_prob[r * top + j] = ((value_in(order) - m) * k - log2s) * kLn2;
+    out.top_log_prob[r * top + j] = (Distance(m, k)(value_in(order)) - log2s) * kLn2;
     out.top_index[r * top + j] = index_in(order);
 }
 
@@ -188,10 +220,10 @@ __global__ void __launch_bounds__(kThreads) token_short_fwd(
         a.m = fmaxf(a.m, v[j]);
     }
     a.m = group_max<LANES>(a.m);
-    float ref = a.m == -INFINITY ? 0.f : a.m;
+    Distance distance(a.m == -INFINITY ? 0.f : a.m, k);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        float d = (v[j] - ref) * k;
+        float d = distance(v[j]);
         float e = __builtin_amdgcn_exp2f(d);
         a.s += e;
         a.t += e * fmaxf(d, kFar);
@@ -228,9 +260,9 @@ __device__ inline void rank_orders(const unsigned long long* orders, int n, int 
     }
 }
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads) token_segment_fwd(
-    Rows rows, const int64_t* __restrict__ index, Out out, int V, int segments, float k, int64_t ignore,
+    Rows rows, const int64_t* __restrict__ index, Out out, int V, int segments, int length, float k, int64_t ignore,
     int has_ignore, int top, float* __restrict__ partial, unsigned long long* __restrict__ offered
 ) {
     constexpr int N = Pack<T>::N;
@@ -243,36 +275,42 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
         return;
     }
     const T* x = row_of<T>(rows, r);
-    int lo = seg * kSegment;
+    int lo = seg * length, hi = min(V, lo + length);
     Pack<T> v[kPerThread / N];
 #pragma unroll
     for (int j = 0; j < kPerThread / N; ++j) {
         int c = lo + (j * kThreads + tid) * N;
-        if (c + N <= V) {
+        if (c + N <= hi) {
             v[j] = load_pack(x + c);
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[j].v[i] = c + i < V ? x[c + i] : from_f<T>(-INFINITY);
+            for (int i = 0; i < N; ++i) v[j].v[i] = c + i < hi ? x[c + i] : from_f<T>(-INFINITY);
         }
     }
     Sums a{-INFINITY, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kPerThread / N; ++j)
 #pragma unroll
-        for (int i = 0; i < N; ++i) a.m = fmaxf(a.m, to_f(v[j].v[i]));
+        for (int i = 0; i < N; i += 2) a.m = fmaxf(a.m, fmaxf(to_f(v[j].v[i]), to_f(v[j].v[i + 1])));
     a.m = group_max<kWave>(a.m);
-    float ref = a.m == -INFINITY ? 0.f : a.m;
+    Distance distance(a.m == -INFINITY ? 0.f : a.m, k);
+    auto add = [&](auto far) {
 #pragma unroll
-    for (int j = 0; j < kPerThread / N; ++j)
+        for (int j = 0; j < kPerThread / N; ++j)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float d = (to_f(v[j].v[i]) - ref) * k;
-            float e = __builtin_amdgcn_exp2f(d);
-            a.s += e;
-            a.t += e * fmaxf(d, kFar);
-        }
+            for (int i = 0; i < N; ++i) {
+                float d = distance.template at<decltype(far)::value>(to_f(v[j].v[i]));
+                float e = __builtin_amdgcn_exp2f(d);
+                a.s += e;
+                if (ENTROPY) a.t += e * fmaxf(d, kFar);
+            }
+    };
+    if (distance.far)
+        add(std::true_type{});
+    else
+        add(std::false_type{});
     a.s = group_sum<kWave>(a.s);
-    a.t = group_sum<kWave>(a.t);
+    if (ENTROPY) a.t = group_sum<kWave>(a.t);
     __shared__ Sums part[kThreads / kWave];
     if (tid % kWave == 0) part[tid / kWave] = a;
 
@@ -289,7 +327,7 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 int c = lo + (j * kThreads + tid) * N + i;
-                unsigned long long o = c < V ? order_of(to_f(v[j].v[i]), c) : 0;
+                unsigned long long o = c < hi ? order_of(to_f(v[j].v[i]), c) : 0;
                 mine = o > mine ? o : mine;
             }
         best[tid] = mine;
@@ -308,7 +346,7 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 int c = lo + (j * kThreads + tid) * N + i;
-                unsigned long long o = c < V ? order_of(to_f(v[j].v[i]), c) : 0;
+                unsigned long long o = c < hi ? order_of(to_f(v[j].v[i]), c) : 0;
                 if (o >= bound) candidates[atomicAdd(&found, 1)] = o;
             }
     }
@@ -337,6 +375,85 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
                 if (j >= found) mine[j] = 0;
             rank_orders(candidates, found, top, [&](int j, unsigned long long o) { mine[j] = o; });
         }
+    }
+}
+
+// A workgroup walks a whole row, the next 8192 logits on their way while it sums the present ones; each thread keeps
+// sums of its own and moves their reference when it meets a larger logit. For many rows: the chip is full then, and
+// segments of their own would spend their time on starting (16384 rows of 131072 bf16 logits, of which three quarters
+// are live: 0.67 ms, 4.8 TB/s, in segments 0.82 ms; 8184 rows of 50001, six tenths live: 102 us against 131).
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(kThreads) token_stream_fwd(
+    Rows rows, const int64_t* __restrict__ index, Out out, int V, float k, int64_t ignore, int has_ignore
+) {
+    constexpr int N = Pack<T>::N, PACKS = kPerThread / N;
+    int64_t r = blockIdx.x;
+    int tid = threadIdx.x;
+    int64_t token = index[r];
+    if (has_ignore && token == ignore) {
+        write_nothing(out, r, 0, tid, kThreads);
+        return;
+    }
+    const T* x = row_of<T>(rows, r);
+    Pack<T> now[PACKS], next[PACKS];
+    auto load = [&](Pack<T>(&v)[PACKS], int lo) {
+        if (lo + kSegment <= V) {
+#pragma unroll
+            for (int j = 0; j < PACKS; ++j) v[j] = load_pack(x + lo + (j * kThreads + tid) * N);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PACKS; ++j) {
+                int c = lo + (j * kThreads + tid) * N;
+                if (c + N <= V) {
+                    v[j] = load_pack(x + c);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) v[j].v[i] = c + i < V ? x[c + i] : from_f<T>(-INFINITY);
+                }
+            }
+        }
+    };
+    Sums a{-INFINITY, 0.f, 0.f};
+    load(now, 0);
+    for (int lo = 0; lo < V; lo += kSegment) {
+        if (lo + kSegment < V) load(next, lo + kSegment);
+        float m = a.m;
+#pragma unroll
+        for (int j = 0; j < PACKS; ++j)
+#pragma unroll
+            for (int i = 0; i < N; i += 2) m = fmaxf(m, fmaxf(to_f(now[j].v[i]), to_f(now[j].v[i + 1])));
+        if (m > a.m) shift(a, m, k);
+        Distance distance(m == -INFINITY ? 0.f : m, k);
+        auto add = [&](auto far) {
+#pragma unroll
+            for (int j = 0; j < PACKS; ++j)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    float d = distance.template at<decltype(far)::value>(to_f(now[j].v[i]));
+                    float e = __builtin_amdgcn_exp2f(d);
+                    a.s += e;
+                    if (ENTROPY) a.t += e * fmaxf(d, kFar);
+                }
+        };
+        if (distance.far)
+            add(std::true_type{});
+        else
+            add(std::false_type{});
+#pragma unroll
+        for (int j = 0; j < PACKS; ++j) now[j] = next[j];
+    }
+    float m = group_max<kWave>(a.m);
+    shift(a, m, k);
+    a.s = group_sum<kWave>(a.s);
+    if (ENTROPY) a.t = group_sum<kWave>(a.t);
+    __shared__ Sums part[kThreads / kWave];
+    if (tid % kWave == 0) part[tid / kWave] = a;
+    __syncthreads();
+    if (tid == 0) {
+        Sums all = part[0];
+#pragma unroll
+        for (int w = 1; w < kThreads / kWave; ++w) all = join(all, part[w], k);
+        write_row(out, r, all, x, token, V, k);
     }
 }
 
@@ -406,9 +523,14 @@ __device__ inline RowGrad row_grad(const Grads& g, int64_t r, int top, int64_t t
     return a;
 }
 
+template <bool FAR, bool ENTROPY>
+__device__ inline float grad_at(const RowGrad& a, const Distance& distance, float x) {
+    float d = distance.at<FAR>(x) - a.log2s, p = __builtin_amdgcn_exp2f(d);
+    return ENTROPY ? p * fmaf(a.c1, fmaxf(d, kFar), a.c0) : p * a.c0;
+}
 __device__ inline float grad_at(const RowGrad& a, float x, float k) {
-    float d = (x - a.m) * k - a.log2s;
-    return __builtin_amdgcn_exp2f(d) * (a.c0 + a.c1 * fmaxf(d, kFar));
+    Distance distance(a.m, k);
+    return distance.far ? grad_at<true, true>(a, distance, x) : grad_at<false, true>(a, distance, x);
 }
 
 // the share of column c alone, and whether lane j is the one that adds it: lanes 0..top-1 stand for the largest
@@ -460,14 +582,14 @@ __global__ void __launch_bounds__(kThreads) token_short_bwd(
     }
 }
 
-template <typename T>
+template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads) token_segment_bwd(
-    Rows rows, const int64_t* __restrict__ index, Grads g, T* __restrict__ grad, int V, int segments, float k,
+    Rows rows, const int64_t* __restrict__ index, Grads g, T* __restrict__ grad, int V, int segments, int length, float k,
     float inv_t, int64_t ignore, int has_ignore, int top
 ) {
     constexpr int N = Pack<T>::N;
     int64_t r = blockIdx.x / segments;
-    int lo = (blockIdx.x % segments) * kSegment;
+    int lo = (blockIdx.x % segments) * length, hi = min(V, lo + length);
     int tid = threadIdx.x;
     int64_t token = index[r];
     T* out = grad + r * V;
@@ -475,25 +597,35 @@ __global__ void __launch_bounds__(kThreads) token_segment_bwd(
     const T* x = row_of<T>(rows, r);
     RowGrad a{0.f, 0.f, 0.f, 0.f};
     if (live) a = row_grad(g, r, top, token, V, inv_t);
+    Distance distance(a.m, k);
+    auto write = [&](auto far) {
+        constexpr bool FAR = decltype(far)::value;
 #pragma unroll
-    for (int j = 0; j < kPerThread / N; ++j) {
-        int c = lo + (j * kThreads + tid) * N;
-        if (c + N <= V) {
-            Pack<T> v, o;
-            if (live) v = load_pack(x + c);
+        for (int j = 0; j < kPerThread / N; ++j) {
+            int c = lo + (j * kThreads + tid) * N;
+            if (c + N <= hi) {
+                Pack<T> v, o;
+                if (live) v = load_pack(x + c);
 #pragma unroll
-            for (int i = 0; i < N; ++i) o.v[i] = from_f<T>(live ? grad_at(a, to_f(v.v[i]), k) : 0.f);
-            store_pack(out + c, o);
-        } else {
-            for (int i = 0; c + i < V; ++i) out[c + i] = from_f<T>(live ? grad_at(a, to_f(x[c + i]), k) : 0.f);
+                for (int i = 0; i < N; ++i)
+                    o.v[i] = from_f<T>(live ? grad_at<FAR, ENTROPY>(a, distance, to_f(v.v[i])) : 0.f);
+                store_pack(out + c, o);
+            } else {
+                for (int i = 0; c + i < hi; ++i)
+                    out[c + i] = from_f<T>(live ? grad_at<FAR, ENTROPY>(a, distance, to_f(x[c + i])) : 0.f);
+            }
         }
-    }
+    };
+    if (distance.far)
+        write(std::true_type{});
+    else
+        write(std::false_type{});
     if (!live) return;
     __syncthreads();  // the single columns are written again, whole, after the others
     int column;
     float share;
     if (tid <= top && own_share(g, r, top, tid, token, V, inv_t, column, share) && column >= lo &&
-        column < lo + kSegment)
+        column < hi)
         out[column] = from_f<T>(grad_at(a, to_f(x[column]), k) + share);
 }
 
@@ -527,6 +659,9 @@ void check_args(const torch::Tensor& logits, const torch::Tensor& index) {
                 "token_log_prob: logits [..., V] and index [...] must be on one HIP device");
     TORCH_CHECK(logits.size(-1) >= 1 && logits.size(-1) <= (1 << 30), "token_log_prob: V must be in [1, 2^30]");
 }
+
+// segments of a row are equally long, in whole packs
+int length_of(int V, int segments) { return ((V + segments - 1) / segments + 7) / 8 * 8; }
 
 template <typename F>
 void by_type(const torch::Tensor& x, F&& f) {
@@ -574,6 +709,11 @@ std::vector<torch::Tensor> token_log_prob_fwd(
         } else if (V <= 512) {
             token_short_fwd<T, 64, 8><<<cdiv(count, kThreads / 64), kThreads, 0, stream>>>(
                 rows, ix, out, count, V, k, ignore, has_ignore, top);
+        } else if (top == 0 && segments > 1 && count >= kManyRows) {
+            if (want_entropy)
+                token_stream_fwd<T, true><<<(unsigned)count, kThreads, 0, stream>>>(rows, ix, out, V, k, ignore, has_ignore);
+            else
+                token_stream_fwd<T, false><<<(unsigned)count, kThreads, 0, stream>>>(rows, ix, out, V, k, ignore, has_ignore);
         } else {
             torch::Tensor partial, offered;
             float* p = nullptr;
@@ -587,12 +727,16 @@ std::vector<torch::Tensor> token_log_prob_fwd(
                 }
             }
             dim3 grid((unsigned)(count * segments));
+            int length = length_of(V, segments);
+            auto go = [&](auto kernel) {
+                kernel<<<grid, kThreads, 0, stream>>>(rows, ix, out, V, segments, length, k, ignore, has_ignore, top, p, o);
+            };
             if (top > 0)
-                token_segment_fwd<T, true><<<grid, kThreads, 0, stream>>>(
-                    rows, ix, out, V, segments, k, ignore, has_ignore, top, p, o);
+                go(token_segment_fwd<T, true, true>);
+            else if (want_entropy)
+                go(token_segment_fwd<T, false, true>);
             else
-                token_segment_fwd<T, false><<<grid, kThreads, 0, stream>>>(
-                    rows, ix, out, V, segments, k, ignore, has_ignore, top, p, o);
+                go(token_segment_fwd<T, false, false>);
             if (segments > 1) {
                 HIP_CHECK_LAST();
                 if (top > 0)
@@ -644,9 +788,13 @@ torch::Tensor token_log_prob_bwd(
         else if (V <= 512)
             token_short_bwd<T, 64><<<cdiv(count, kThreads / 64), kThreads, 0, stream>>>(
                 rows, ix, g, to, count, V, k, inv_t, ignore, has_ignore, top);
-        else
-            token_segment_bwd<T><<<(unsigned)(count * segments), kThreads, 0, stream>>>(
-                rows, ix, g, to, V, segments, k, inv_t, ignore, has_ignore, top);
+        else {
+            auto go = [&](auto kernel) {
+                kernel<<<(unsigned)(count * segments), kThreads, 0, stream>>>(
+                    rows, ix, g, to, V, segments, length_of(V, segments), k, inv_t, ignore, has_ignore, top);
+            };
+            g.entropy ? go(token_segment_bwd<T, true>) : go(token_segment_bwd<T, false>);
+        }
     });
     HIP_CHECK_LAST();
     return grad;

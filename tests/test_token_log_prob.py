@@ -78,6 +78,8 @@ def close(got, want, tol, name=''):
     got = got.detach().cpu()
     half = 0.0 if got.dtype in (torch.float32, torch.float64) else torch.finfo(got.dtype).eps / 2
     floor = 2.0 ** -25 if got.dtype == torch.float16 else 2.0 ** -126
+    # a value beyond the type's largest number rounds to infinity
+    want = torch.where(want.abs() > torch.finfo(got.dtype).max, want.sign() * float('inf'), want)
     got = got.double()
     bad = ~((got - want).abs() <= tol + half * (want.abs() + tol) + floor)
     both = (torch.isnan(got) & torch.isnan(want)) | (torch.isinf(want) & (got == want))
@@ -250,6 +252,33 @@ def test_gpu_ignored_rows(V):
     assert torch.equal(token_log_prob(logits, index, ignore_index=-100).log_prob[3], torch.zeros(6, device='cuda'))
     index[:] = 0
     check(logits.nan_to_num(), index, 1.0, 0, 2)
+
+
+@gpu
+@pytest.mark.parametrize('V', [8193, 16384, 17003])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_gpu_many_rows(V, dtype):
+    rows = 1030  # enough for a workgroup to walk a row of its own
+    logits = torch.empty(rows, V, dtype=dtype, device='cuda').normal_(0, 3)
+    logits[:, 8190::7] = float('-inf')
+    logits[1, :8192] = float('-inf')  # nothing but masked tokens at first
+    logits[2] = torch.finfo(dtype).min
+    logits[3, :8192] = torch.finfo(dtype).min
+    logits[4] = torch.linspace(-40, 40, V, device='cuda').to(dtype)  # the maximum moves all the time
+    logits[5, 5] = float('nan')
+    logits[6] = float('-inf')
+    index = torch.randint(0, V // 8, (rows, ), device='cuda') * 7
+    index[7::5] = -100
+    index[1] = 8193 - 1 if V == 8193 else 8193
+    index[2:5] = 3
+    got = token_log_prob(logits, index, 0.8, -100, True)
+    assert torch.isnan(got.log_prob[5:7]).all() and torch.isnan(got.entropy[5:7]).all()
+    keep = [0, 1, 2, 3, 4, 7, 8, 9, 500, rows - 2, rows - 1]
+    want, tol = oracle(logits[keep], index[keep], 0.8, -100)
+    close(got.log_prob[keep], want['log_prob'], tol['log_prob'], 'log_prob')
+    close(got.entropy[keep], want['entropy'], tol['entropy'], 'entropy')
+    alone = token_log_prob(logits, index, 0.8, -100).log_prob  # without the entropy
+    assert torch.equal(alone.nan_to_num(), got.log_prob.nan_to_num())
 
 
 @gpu
