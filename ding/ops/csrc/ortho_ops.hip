@@ -221,11 +221,14 @@ struct Epilogue {
 //   UPDATE:    A = X^T, B symmetric: C = (B X)^T; x <- beta x + C^T, its transpose to out. x may have one plane on the
 //              way in (PA) and has two on the way out.
 //   LAST:      the same, written to the caller's matrix in its type.
+// Two symmetric products with the same A go in one launch: behind the first `matrices` of the grid's depth are those of
+// the second B and out.
 // A stage of 32 columns is copied straight into LDS while the one before it is multiplied. Within a row of a stage the
 // four 16-byte pieces change places with the row, so that eight rows read at once fall into different banks.
 template <typename P, Kind kind, int PA, int PB>
 __global__ void __launch_bounds__(P::THREADS) product_kernel(
-    Split a, Split bm, int depth, Epilogue ep, Split x, Split out, Target to
+    Split a, Split bm, int depth, Epilogue ep, Split x, Split out, Target to, int matrices, Split second_b,
+    Split second_out
 ) {
     typedef Mfma<P::SIDE> M;
     constexpr int TILE = P::TILE, SIDE = P::SIDE, SI = P::WM / SIDE, SJ = P::WN / SIDE;
@@ -243,6 +246,11 @@ __global__ void __launch_bounds__(P::THREADS) product_kernel(
         bj = blockIdx.y;
     }
     int64_t batch = blockIdx.z;
+    if (kind == SYMMETRIC && (int)blockIdx.z >= matrices) {
+        batch -= matrices;
+        bm = second_b;
+        out = second_out;
+    }
     int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     int wi = wave / (TILE / P::WN) * P::WM, wj = wave % (TILE / P::WN) * P::WN;
     typename M::Acc acc[SI][SJ];
@@ -425,6 +433,240 @@ __global__ void __launch_bounds__(P::THREADS) product_kernel(
             }
 }
 
+// ------------------------------------------------------------------------------------------------ small matrices
+// A matrix of up to 128 x 256 has a workgroup of its own for the whole iteration: X stays in registers in 32 bits, its
+// factors and G's lie in LDS, and nothing is launched or stored between the products, where a launch of its own takes
+// about 5 us a product whatever its size. Up to 256 matrices of 64 x 64 take 15 us, of 128 x 128 56 us (six of them by
+// launches: 95 us). Of 128 x 256 they take 108 us, six of them by launches 104 us, 64 of them 160 us.
+// X is held as the results of (B X)^T: rows r of X^T in parts of kPart, columns c; a wave has a half of a part's rows
+// and a quarter of the columns. The same place in LDS holds X and X^T in turns, a part at a time.
+struct Small {
+    float gram, square, linear, update, keep;  // factors of C in G, of C and G in B, of C and x in x
+    float scale, inv_scale;
+    double eps;
+    int steps;
+};
+
+template <int MP, int NP>
+struct SmallShape {
+    static constexpr int PART = NP < 128 ? NP : 128, PARTS = NP / PART;
+    static constexpr int WAVES = 8, THREADS = WAVES * kWave;
+    static constexpr int XI = PART / 2 / 16, GI = MP / 2 / 16, J = MP / 4 / 16;
+    static constexpr int X_PLANE = MP * PART, G_PLANE = MP * MP;  // halves
+};
+
+// where element (row, k) of a plane of `rows` rows lies: panels of 32 columns, pieces changing places with the row
+__device__ inline int small_at(int rows, int row, int k) {
+    return (k / 32 * rows + row) * 32 + (((k / 8) & 3) ^ ((row >> 1) & 3)) * 8 + k % 8;
+}
+
+template <typename T, int MP, int NP>
+__global__ void __launch_bounds__(512) small_kernel(Matrix m, Target to, Small p) {
+    typedef SmallShape<MP, NP> S;
+    typedef Mfma<16> M;
+    __shared__ __attribute__((aligned(16))) _Float16 lx[2 * S::X_PLANE], lg[2 * S::G_PLANE];
+    __shared__ double part[S::WAVES];
+    int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    int r_wave = wave / 4, c0 = wave % 4 * (MP / 4) + lane % 16, r_lane = lane / 16 * 4;
+    auto row_x = [&](int q, int i) { return q * S::PART + r_wave * (S::PART / 2) + i * 16 + r_lane; };
+    float x[S::PARTS][S::XI][S::J][4];
+    double sum = 0;
+#pragma unroll
+    for (int q = 0; q < S::PARTS; ++q)
+#pragma unroll
+        for (int i = 0; i < S::XI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    int r = row_x(q, i) + e, c = c0 + j * 16;
+                    float v = 0.f;
+                    if (c < m.rows && r < m.cols)
+                        v = to_f(((const T*)m.base)[blockIdx.x * m.batch_stride + c * m.row_stride + r * m.col_stride]);
+                    x[q][i][j][e] = v;
+                    sum += (double)v * v;
+                }
+    for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+    if (lane == 0) part[wave] = sum;
+    __syncthreads();
+    sum = part[0];
+    for (int w = 1; w < S::WAVES; ++w) sum += part[w];
+    double factor = p.scale / (sqrt(sum) + p.eps);
+    // a matrix of numbers below 2^-126 takes a factor that 32 bits do not hold: it goes in two steps
+    float first = (float)fmin(factor, 0x1p100), second = (float)(factor / first);
+#pragma unroll
+    for (int q = 0; q < S::PARTS; ++q)
+#pragma unroll
+        for (int i = 0; i < S::XI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[q][i][j][e] = x[q][i][j][e] * first * second;
+
+    // acc[i][j] += rows `ra` of A times rows `rb` of B, over `depth` columns; planes lie behind each other
+    auto multiply = [&](auto& acc, const _Float16* a, int a_rows, int ra, const _Float16* b, int b_rows, int depth) {
+        constexpr int I = sizeof(acc) / sizeof(acc[0]);
+        for (int k = 0; k < depth; k += 32) {
+            half8 fa[2][I], fb[2][S::J];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < I; ++i)
+                    fa[h][i] = *(const half8*)(a + h * a_rows * depth +
+                                               small_at(a_rows, ra + i * 16 + lane % 16, k + lane / 16 * 8));
+#pragma unroll
+                for (int j = 0; j < S::J; ++j)
+                    fb[h][j] = *(const half8*)(b + h * b_rows * depth +
+                                               small_at(b_rows, c0 + j * 16, k + lane / 16 * 8));
+            }
+#pragma unroll
+            for (int t = 0; t < 3; ++t)
+#pragma unroll
+                for (int i = 0; i < I; ++i)
+#pragma unroll
+                    for (int j = 0; j < S::J; ++j) acc[i][j] = M::run(fa[t == 0][i], fb[t == 1][j], acc[i][j]);
+        }
+    };
+
+    for (int step = 0; step < p.steps; ++step) {
+        // G, a part of X's columns at a time
+        float4v acc[S::GI][S::J];
+#pragma unroll
+        for (int i = 0; i < S::GI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::J; ++j) acc[i][j] = (float4v)(0.f);
+#pragma unroll
+        for (int q = 0; q < S::PARTS; ++q) {
+            if (q > 0) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < S::XI; ++i)
+#pragma unroll
+                for (int j = 0; j < S::J; ++j) {
+                    half4 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        _Float16 h, l;
+                        split(x[q][i][j][e], h, l);
+                        hi[e] = h, lo[e] = l;
+                    }
+                    int at = small_at(MP, c0 + j * 16, row_x(0, i));
+                    *(half4*)(lx + at) = hi;
+                    *(half4*)(lx + S::X_PLANE + at) = lo;
+                }
+            __syncthreads();
+            multiply(acc, lx, MP, r_wave * (MP / 2), lx, MP, S::PART);
+        }
+        // G is symmetric: its element (r, c) is written as (c, r)
+        auto place = [&](int i, int j) { return small_at(MP, c0 + j * 16, r_wave * (MP / 2) + i * 16 + r_lane); };
+        auto write_g = [&] {
+#pragma unroll
+            for (int i = 0; i < S::GI; ++i)
+#pragma unroll
+                for (int j = 0; j < S::J; ++j) {
+                    half4 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        _Float16 h, l;
+                        split(acc[i][j][e], h, l);
+                        hi[e] = h, lo[e] = l;
+                    }
+                    *(half4*)(lg + place(i, j)) = hi;
+                    *(half4*)(lg + S::G_PLANE + place(i, j)) = lo;
+                }
+        };
+        float kept[S::GI][S::J][4];
+#pragma unroll
+        for (int i = 0; i < S::GI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc[i][j][e] *= p.gram;
+                    kept[i][j][e] = p.linear * acc[i][j][e];
+                }
+        write_g();
+        __syncthreads();
+        // B = b G + c G G in the place of G
+#pragma unroll
+        for (int i = 0; i < S::GI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::J; ++j) acc[i][j] = (float4v)(0.f);
+        multiply(acc, lg, MP, r_wave * (MP / 2), lg, MP, MP);
+#pragma unroll
+        for (int i = 0; i < S::GI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = acc[i][j][e] * p.square + kept[i][j][e];
+        __syncthreads();
+        write_g();
+        // x <- a x + (B X)^T, a part of X^T's rows at a time
+#pragma unroll
+        for (int q = 0; q < S::PARTS; ++q) {
+            if (q > 0) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < S::XI; ++i)
+#pragma unroll
+                for (int j = 0; j < S::J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        _Float16 h, l;
+                        split(x[q][i][j][e], h, l);
+                        int at = small_at(S::PART, row_x(0, i) + e, c0 + j * 16);
+                        lx[at] = h;
+                        lx[S::X_PLANE + at] = l;
+                    }
+            __syncthreads();
+            float4v got[S::XI][S::J];
+#pragma unroll
+            for (int i = 0; i < S::XI; ++i)
+#pragma unroll
+                for (int j = 0; j < S::J; ++j) got[i][j] = (float4v)(0.f);
+            multiply(got, lx, S::PART, r_wave * (S::PART / 2), lg, MP, MP);
+#pragma unroll
+            for (int i = 0; i < S::XI; ++i)
+#pragma unroll
+                for (int j = 0; j < S::J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[q][i][j][e] = p.keep * x[q][i][j][e] + p.update * got[i][j][e];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int q = 0; q < S::PARTS; ++q)
+#pragma unroll
+        for (int i = 0; i < S::XI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    int r = row_x(q, i) + e, c = c0 + j * 16;
+                    if (c < to.rows && r < to.cols)
+                        ((T*)to.base)[blockIdx.x * to.batch_stride + c * to.row_stride + r * to.col_stride] =
+                            from_f<T>(x[q][i][j][e] * p.inv_scale);
+                }
+}
+
+// whether a small kernel takes it; if so it is launched
+template <typename T>
+bool small_run(const Matrix& in, const Target& to, const Small& p, int64_t batch, hipStream_t stream) {
+    auto go = [&](auto mp, auto np) {
+        constexpr int MP = decltype(mp)::value, NP = decltype(np)::value;
+        small_kernel<T, MP, NP><<<(unsigned)batch, 512, 0, stream>>>(in, to, p);
+        return true;
+    };
+    if (in.rows > 64 && in.cols > 128 && batch < 16) return false;
+    auto wide = [&](auto mp) {
+        if (in.cols <= 64 && decltype(mp)::value == 64) return go(mp, std::integral_constant<int, 64>{});
+        if (in.cols <= 128) return go(mp, std::integral_constant<int, 128>{});
+        if (in.cols <= 256) return go(mp, std::integral_constant<int, 256>{});
+        return false;
+    };
+    if (in.rows <= 64) return wide(std::integral_constant<int, 64>{});
+    if (in.rows <= 128) return wide(std::integral_constant<int, 128>{});
+    return false;
+}
+
 template <typename F>
 void by_type(const torch::Tensor& x, F&& f) {
     switch (x.scalar_type()) {
@@ -492,18 +734,28 @@ torch::Tensor newton_schulz(
     int64_t batch = matrices.size(0), rows = matrices.size(1), cols = matrices.size(2);
     bool tall = rows > cols;
     int64_t m = tall ? cols : rows, n = tall ? rows : cols;
-    TORCH_CHECK(steps >= 1 && batch < 65536 && n <= (1 << 20) && scales.size() == 5,
-                "orthogonalize: at least one step, fewer than 65536 matrices and sides of up to 2^20");
+    TORCH_CHECK(steps >= 1 && batch < 32768 && n <= (1 << 20) && scales.size() == 5,
+                "orthogonalize: at least one step, fewer than 32768 matrices and sides of up to 2^20");
     double sx = scales[0], sg = scales[1], sb = scales[2], sq = scales[3], sp = scales[4];
-    int lower = side_of(m, m, batch, true), rect = side_of(m, n, batch, false);
+    int lower = side_of(m, m, batch, true), both = side_of(m, m, 2 * batch, true), rect = side_of(m, n, batch, false);
     // rows that tiles of either side reach, and whole tiles of the packing kernel
-    int64_t mp = std::max({up(m, lower), up(m, rect), up(m, kEdge)}), np = std::max(up(n, rect), up(n, kEdge));
+    int64_t mp = std::max({up(m, lower), up(m, both), up(m, rect), up(m, kEdge)}), np = std::max(up(n, rect), up(n, kEdge));
     int depth_m = (int)up(m, kStage), depth_n = (int)up(n, kStage);
     Matrix in{matrices.data_ptr(), matrices.stride(0), matrices.stride(tall ? 2 : 1), matrices.stride(tall ? 1 : 2),
               (int)m, (int)n};
     int type = matrices.scalar_type() == torch::kFloat32 ? 0 : matrices.scalar_type() == torch::kFloat16 ? 1 : 2;
     Target to{result.data_ptr(), result.stride(0), result.stride(tall ? 2 : 1), result.stride(tall ? 1 : 2), (int)m,
               (int)n, type};
+    hipStream_t stream = ding_current_stream();
+    Small small{(float)(sg / (sx * sx)), (float)(c * sb / (sg * sg)), (float)(b * sb / sg), (float)(1.0 / sb), (float)a,
+                (float)sx, (float)(1.0 / sx), eps, (int)steps};
+    bool done = false;
+    by_type(matrices, [&](auto* null) {
+        using T = std::remove_pointer_t<decltype(null)>;
+        done = small_run<T>(in, to, small, batch, stream);
+    });
+    HIP_CHECK_LAST();
+    if (done) return result;
     auto half = matrices.options().dtype(torch::kFloat16);
     int parts = (int)std::min<int64_t>(kNormBlocks, std::max<int64_t>(1, m * n / (kThreads * 16)));
     auto partial = torch::empty({batch * parts}, matrices.options().dtype(torch::kFloat64));
@@ -516,7 +768,6 @@ torch::Tensor newton_schulz(
     };
     bool one = type != 0;  // X has one plane until it is updated
     Split x = planes(mp, np), xt = planes(np, mp), g = planes(mp, mp), q = planes(mp, mp);
-    hipStream_t stream = ding_current_stream();
     by_type(matrices, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
         int64_t dense = std::min(in.row_stride, in.col_stride), line = std::max(in.row_stride, in.col_stride);
@@ -531,16 +782,23 @@ torch::Tensor newton_schulz(
                                                       rest.data_ptr<float>());
         HIP_CHECK_LAST();
     });
-    // out = (alpha A B^T + beta E) scaled, for symmetric results
-    auto symmetric = [&](Split u, Split v, int depth, Epilogue ep, Split e, Split out, bool single) {
-        by_side(lower, tiles_of(m, m, batch, true, lower), [&](auto shape) {
+    // out = (alpha A B^T + beta E) scaled, for symmetric results; with a second B and out if given
+    auto symmetric = [&](Split u, Split v, int depth, Epilogue ep, Split e, Split out, bool single,
+                         const Split* v2 = nullptr, const Split* out2 = nullptr) {
+        int64_t count = v2 ? 2 * batch : batch;
+        int side = side_of(m, m, count, true);
+        by_side(side, tiles_of(m, m, count, true, side), [&](auto shape) {
             using P = decltype(shape);
             unsigned r = (unsigned)up(m, P::TILE) / P::TILE;
-            dim3 grid(r * (r + 1) / 2, 1, (unsigned)batch);
+            dim3 grid(r * (r + 1) / 2, 1, (unsigned)count);
+            auto go = [&](auto kernel) {
+                kernel<<<grid, P::THREADS, 0, stream>>>(u, v, depth, ep, e, out, to, (int)batch, v2 ? *v2 : v,
+                                                        out2 ? *out2 : out);
+            };
             if (single)
-                product_kernel<P, SYMMETRIC, 1, 1><<<grid, P::THREADS, 0, stream>>>(u, v, depth, ep, e, out, to);
+                go(product_kernel<P, SYMMETRIC, 1, 1>);
             else
-                product_kernel<P, SYMMETRIC, 2, 2><<<grid, P::THREADS, 0, stream>>>(u, v, depth, ep, e, out, to);
+                go(product_kernel<P, SYMMETRIC, 2, 2>);
         });
         HIP_CHECK_LAST();
     };
@@ -552,7 +810,7 @@ torch::Tensor newton_schulz(
             using P = decltype(shape);
             dim3 grid((unsigned)up(n, P::TILE) / P::TILE, (unsigned)up(m, P::TILE) / P::TILE, (unsigned)batch);
             auto go = [&](auto kernel) {
-                kernel<<<grid, P::THREADS, 0, stream>>>(xt, p, depth_m, ep, x, next, to);
+                kernel<<<grid, P::THREADS, 0, stream>>>(xt, p, depth_m, ep, x, next, to, (int)batch, p, next);
             };
             if (last)
                 one ? go(product_kernel<P, LAST, 1, 2>) : go(product_kernel<P, LAST, 2, 2>);
@@ -589,14 +847,16 @@ torch::Tensor newton_schulz(
             symmetric(g, g, depth_m,
                       {(float)(c * s_into / (sg * sg)), (float)(b * s_into / sg), (float)(a * s_into), nullptr, 0, 0, 0.f},
                       g, into, false);
-            if (i > 0) {
-                symmetric(q, p[(i + 1) % 2], depth_m, {(float)(1.0 / sq), 0.f, 0.f, nullptr, 0, 0, 0.f}, g, p[i % 2],
-                          false);
-            }
-            if (i + 1 < count) {
-                symmetric(into, g, depth_m, {(float)(1.0 / s_into), 0.f, 0.f, nullptr, 0, 0, 0.f}, g, y, false);
-                symmetric(y, into, depth_m, {(float)(1.0 / s_into), 0.f, 0.f, nullptr, 0, 0, 0.f}, g, g, false);
-            }
+            Epilogue plain{(float)(1.0 / s_into), 0.f, 0.f, nullptr, 0, 0, 0.f};
+            bool more = i + 1 < count;
+            // P <- Q P and Y = Q G, together where both are wanted; then G <- Y Q
+            if (i > 0 && more)
+                symmetric(q, g, depth_m, plain, g, y, false, &p[(i + 1) % 2], &p[i % 2]);
+            else if (i > 0)
+                symmetric(q, p[(i + 1) % 2], depth_m, plain, g, p[i % 2], false);
+            else if (more)
+                symmetric(into, g, depth_m, plain, g, y, false);
+            if (more) symmetric(y, into, depth_m, plain, g, g, false);
         }
         update(p[(count + 1) % 2], sp, 0.0, s + count == steps, next);
     }
