@@ -216,149 +216,25 @@ struct Epilogue {
     float inv_scale;
 };
 
-// C = A B^T over split factors of PA and PB planes, a TILE x TILE tile a workgroup.
-//   SYMMETRIC: C is symmetric: tiles of the lower triangle, written twice. E = x where beta is not 0.
-//   UPDATE:    A = X^T, B symmetric: C = (B X)^T; x <- beta x + C^T, its transpose to out. x may have one plane on the
-//              way in (PA) and has two on the way out.
-//   LAST:      the same, written to the caller's matrix in its type.
-// Two symmetric products with the same A go in one launch: behind the first `matrices` of the grid's depth are those of
-// the second B and out.
-// A stage of 32 columns is copied straight into LDS while the one before it is multiplied. Within a row of a stage the
-// four 16-byte pieces change places with the row, so that eight rows read at once fall into different banks.
-template <typename P, Kind kind, int PA, int PB>
-__global__ void __launch_bounds__(P::THREADS) product_kernel(
-    Split a, Split bm, int depth, Epilogue ep, Split x, Split out, Target to, int matrices, Split second_b,
-    Split second_out
+// The sums of a tile, as a wave's lanes hold them.
+template <typename P>
+struct Sums {
+    typedef Mfma<P::SIDE> M;
+    static constexpr int SI = P::WM / P::SIDE, SJ = P::WN / P::SIDE;
+    typename M::Acc acc[SI][SJ];
+};
+
+// What becomes of the sums of tile (bi, bj).
+template <typename P, Kind kind, int PA>
+__device__ inline void finish(
+    const Sums<P>& sums, int bi, int bj, int64_t batch, const Epilogue& ep, const Split& x, const Split& out,
+    const Target& to
 ) {
     typedef Mfma<P::SIDE> M;
-    constexpr int TILE = P::TILE, SIDE = P::SIDE, SI = P::WM / SIDE, SJ = P::WN / SIDE;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[P::STAGES][(PA + PB) * P::PLANE];
-    int bi, bj;
-    if constexpr (kind == SYMMETRIC) {
-        // Workgroups go to the eight dies in turn: each die takes neighbouring tiles of the lower triangle, whose
-        // factors meet in its cache (three of 1001: a tenth of the time; rectangles lost a third of theirs by it).
-        int t = blockIdx.x, die = t % 8, each = gridDim.x / 8, over = gridDim.x % 8;
-        t = die * each + min(die, over) + t / 8;
-        bi = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-        while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
-        while (bi * (bi + 1) / 2 > t) --bi;
-        bj = t - bi * (bi + 1) / 2;
-    } else {
-        bi = blockIdx.x;
-        bj = blockIdx.y;
-    }
-    int64_t batch = blockIdx.z;
-    if (kind == SYMMETRIC && (int)blockIdx.z >= matrices) {
-        batch -= matrices;
-        bm = second_b;
-        out = second_out;
-    }
+    constexpr int TILE = P::TILE, SIDE = P::SIDE, SI = Sums<P>::SI, SJ = Sums<P>::SJ;
     int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     int wi = wave / (TILE / P::WN) * P::WM, wj = wave % (TILE / P::WN) * P::WN;
-    typename M::Acc acc[SI][SJ];
-#pragma unroll
-    for (int i = 0; i < SI; ++i)
-#pragma unroll
-        for (int j = 0; j < SJ; ++j) acc[i][j] = (typename M::Acc)(0.f);
-
-    // a wave copies 16 rows of a plane at a time: lane l takes piece l % 4 of row l / 4, from where it belongs
-    constexpr int GROUPS = (PA + PB) * TILE / 16, COPIES = (GROUPS + P::WAVES - 1) / P::WAVES;
-    const _Float16* from[COPIES];
-    int place[COPIES], pitch[COPIES];
-#pragma unroll
-    for (int c = 0; c < COPIES; ++c) {
-        int group = min(c * P::WAVES + wave, GROUPS - 1);  // every wave issues as many: some copy the last group again
-        int plane = group / (TILE / 16), first = group % (TILE / 16) * 16, row = first + lane / 4;
-        int piece = (lane % 4) ^ P::turn(row);
-        const Split& f = plane < PA ? a : bm;
-        from[c] = ((plane < PA ? plane : plane - PA) ? f.lo : f.hi) +
-                  f.at(batch, (plane < PA ? bi : bj) * TILE + row, piece * 8);
-        pitch[c] = f.rows;
-        place[c] = plane * P::PLANE + first * kStage;
-    }
-    auto fetch = [&](int k0, _Float16* stage) {
-#pragma unroll
-        for (int c = 0; c < COPIES; ++c)
-            copy_to_lds(from[c] + (int64_t)k0 * pitch[c], stage + place[c]);
-    };
-    struct Factors {
-        half8 a[PA][SI], b[PB][SJ];
-    };
-    auto read = [&](Factors& f, const _Float16* stage, int ks) {
-        int piece = ks * (M::DEPTH / 8) + lane / SIDE;
-        auto at = [&](int plane, int r) {
-            return *(const half8*)(stage + plane * P::PLANE + r * kStage + (piece ^ P::turn(r)) * 8);
-        };
-#pragma unroll
-        for (int p = 0; p < PA; ++p)
-#pragma unroll
-            for (int s = 0; s < SI; ++s) f.a[p][s] = at(p, wi + s * SIDE + lane % SIDE);
-#pragma unroll
-        for (int p = 0; p < PB; ++p)
-#pragma unroll
-            for (int s = 0; s < SJ; ++s) f.b[p][s] = at(PA + p, wj + s * SIDE + lane % SIDE);
-    };
-    auto multiply = [&](const Factors& f) {
-        auto all = [&](const half8(&u)[SI], const half8(&v)[SJ]) {
-#pragma unroll
-            for (int i = 0; i < SI; ++i)
-#pragma unroll
-                for (int j = 0; j < SJ; ++j) acc[i][j] = M::run(u[i], v[j], acc[i][j]);
-        };
-        if constexpr (PA == 2) all(f.a[1], f.b[0]);
-        if constexpr (PB == 2) all(f.a[0], f.b[1]);
-        all(f.a[0], f.b[0]);
-        // the next factors' reads are spread between these products
-        constexpr int READS = PA * SI + PB * SJ, PRODUCTS = SI * SJ * (PA + PB - 1);
-#pragma unroll
-        for (int i = 0; i < READS; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / READS > 0 ? PRODUCTS / READS : 1, 0);
-        }
-    };
-    // The factors of the next product are read from LDS while the present ones are multiplied. Copies of a wave arrive
-    // in the order of their issue: when only those of the S - 2 later stages are out, the next stage's are there; after
-    // the barrier everyone's are, and everyone has read the present stage, which is overwritten then.
-    constexpr int S = P::STAGES, STEPS = kStage / M::DEPTH;
-    int stages = depth / kStage, now = 0;
-    Factors even, odd;
-    auto turn_stage = [&](int k, Factors& f) {
-        if (stages - k >= S)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * COPIES) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (k + S < stages) fetch((k + S) * kStage, lds[now]);
-        now = now + 1 == S ? 0 : now + 1;
-        read(f, lds[now], 0);  // behind the last stage it reads what is there, and nobody uses it
-    };
-#pragma unroll
-    for (int k = 0; k < S; ++k)
-        if (k < stages) fetch(k * kStage, lds[k]);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    read(even, lds[0], 0);
-    if constexpr (STEPS == 2) {
-        for (int k = 0; k < stages; ++k) {
-            read(odd, lds[now], 1);
-            multiply(even);
-            turn_stage(k, even);
-            multiply(odd);
-        }
-    } else if constexpr (P::TILE == 192) {
-        // two sets of factors do not fit in registers beside the sums
-        for (int k = 0; k < stages; ++k) {
-            multiply(even);
-            turn_stage(k, even);
-        }
-    } else {
-        for (int k = 0; k < stages; k += 2) {
-            turn_stage(k, odd);
-            multiply(even);
-            if (k + 1 == stages) break;
-            turn_stage(k + 1, even);
-            multiply(odd);
-        }
-    }
-
+    const auto& acc = sums.acc;
     float alpha = ep.alpha, beta = ep.beta;
     if (ep.rest) {
         float r = ep.rest[batch];
@@ -433,6 +309,214 @@ __global__ void __launch_bounds__(P::THREADS) product_kernel(
                     out.lo[at] = lo[e];
                 }
             }
+}
+
+// tile number t of the lower triangle
+__device__ inline void triangle(int t, int& bi, int& bj) {
+    bi = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
+    while (bi * (bi + 1) / 2 > t) --bi;
+    bj = t - bi * (bi + 1) / 2;
+}
+
+// C = A B^T over split factors of PA and PB planes, a TILE x TILE tile a workgroup.
+//   SYMMETRIC: C is symmetric: tiles of the lower triangle, written twice. E = x where beta is not 0.
+//   UPDATE:    A = X^T, B symmetric: C = (B X)^T; x <- beta x + C^T, its transpose to out. x may have one plane on the
+//              way in (PA) and has two on the way out.
+//   LAST:      the same, written to the caller's matrix in its type.
+// Two symmetric products with the same A go in one launch: behind the first `matrices` of the grid's depth are those of
+// the second B and out. A symmetric product may also be cut along its depth, gridDim.y parts of it: the parts' sums go to
+// `partial` and join_kernel adds them up. That fills the chip where tiles are few, and keeps the sums of a long depth
+// short: 130 x 8000 in single precision is 3.6e-6 off without.
+// A stage of 32 columns is copied straight into LDS while the one before it is multiplied. Within a row of a stage the
+// four 16-byte pieces change places with the row, so that eight rows read at once fall into different banks.
+template <typename P, Kind kind, int PA, int PB>
+__global__ void __launch_bounds__(P::THREADS) product_kernel(
+    Split a, Split bm, int depth, Epilogue ep, Split x, Split out, Target to, int matrices, Split second_b,
+    Split second_out, float* __restrict__ partial
+) {
+    typedef Mfma<P::SIDE> M;
+    constexpr int TILE = P::TILE, SIDE = P::SIDE, SI = Sums<P>::SI, SJ = Sums<P>::SJ;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[P::STAGES][(PA + PB) * P::PLANE];
+    int bi, bj, t = blockIdx.x;
+    if constexpr (kind == SYMMETRIC) {
+        // Workgroups go to the eight dies in turn: each die takes neighbouring tiles of the lower triangle, whose
+        // factors meet in its cache (three of 1001: a tenth of the time; rectangles lost a third of theirs by it).
+        int die = t % 8, each = gridDim.x / 8, over = gridDim.x % 8;
+        t = die * each + min(die, over) + t / 8;
+        triangle(t, bi, bj);
+    } else {
+        bi = blockIdx.x;
+        bj = blockIdx.y;
+    }
+    int64_t batch = blockIdx.z;
+    if (kind == SYMMETRIC && (int)blockIdx.z >= matrices) {
+        batch -= matrices;
+        bm = second_b;
+        out = second_out;
+    }
+    int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    int wi = wave / (TILE / P::WN) * P::WM, wj = wave % (TILE / P::WN) * P::WN;
+    Sums<P> sums;
+    auto& acc = sums.acc;
+#pragma unroll
+    for (int i = 0; i < SI; ++i)
+#pragma unroll
+        for (int j = 0; j < SJ; ++j) acc[i][j] = (typename M::Acc)(0.f);
+
+    // a wave copies 16 rows of a plane at a time: lane l takes piece l % 4 of row l / 4, from where it belongs
+    constexpr int GROUPS = (PA + PB) * TILE / 16, COPIES = (GROUPS + P::WAVES - 1) / P::WAVES;
+    const _Float16* from[COPIES];
+    int place[COPIES], pitch[COPIES];
+#pragma unroll
+    for (int c = 0; c < COPIES; ++c) {
+        int group = min(c * P::WAVES + wave, GROUPS - 1);  // every wave issues as many: some copy the last group again
+        int plane = group / (TILE / 16), first = group % (TILE / 16) * 16, row = first + lane / 4;
+        int piece = (lane % 4) ^ P::turn(row);
+        const Split& f = plane < PA ? a : bm;
+        from[c] = ((plane < PA ? plane : plane - PA) ? f.lo : f.hi) +
+                  f.at(batch, (plane < PA ? bi : bj) * TILE + row, piece * 8);
+        pitch[c] = f.rows;
+        place[c] = plane * P::PLANE + first * kStage;
+    }
+    auto fetch = [&](int k0, _Float16* stage) {
+#pragma unroll
+        for (int c = 0; c < COPIES; ++c)
+            copy_to_lds(from[c] + (int64_t)k0 * pitch[c], stage + place[c]);
+    };
+    struct Factors {
+        half8 a[PA][SI], b[PB][SJ];
+    };
+    auto read = [&](Factors& f, const _Float16* stage, int ks) {
+        int piece = ks * (M::DEPTH / 8) + lane / SIDE;
+        auto at = [&](int plane, int r) {
+            return *(const half8*)(stage + plane * P::PLANE + r * kStage + (piece ^ P::turn(r)) * 8);
+        };
+#pragma unroll
+        for (int p = 0; p < PA; ++p)
+#pragma unroll
+            for (int s = 0; s < SI; ++s) f.a[p][s] = at(p, wi + s * SIDE + lane % SIDE);
+#pragma unroll
+        for (int p = 0; p < PB; ++p)
+#pragma unroll
+            for (int s = 0; s < SJ; ++s) f.b[p][s] = at(PA + p, wj + s * SIDE + lane % SIDE);
+    };
+    auto multiply = [&](const Factors& f) {
+        auto all = [&](const half8(&u)[SI], const half8(&v)[SJ]) {
+#pragma unroll
+            for (int i = 0; i < SI; ++i)
+#pragma unroll
+                for (int j = 0; j < SJ; ++j) acc[i][j] = M::run(u[i], v[j], acc[i][j]);
+        };
+        if constexpr (PA == 2) all(f.a[1], f.b[0]);
+        if constexpr (PB == 2) all(f.a[0], f.b[1]);
+        all(f.a[0], f.b[0]);
+        // the next factors' reads are spread between these products
+        constexpr int READS = PA * SI + PB * SJ, PRODUCTS = SI * SJ * (PA + PB - 1);
+#pragma unroll
+        for (int i = 0; i < READS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / READS > 0 ? PRODUCTS / READS : 1, 0);
+        }
+    };
+    // The factors of the next product are read from LDS while the present ones are multiplied. Copies of a wave arrive
+    // in the order of their issue: when only those of the S - 2 later stages are out, the next stage's are there; after
+    // the barrier everyone's are, and everyone has read the present stage, which is overwritten then.
+    constexpr int S = P::STAGES, STEPS = kStage / M::DEPTH;
+    int stages = depth / kStage, now = 0;
+    if (kind == SYMMETRIC && gridDim.y > 1) {
+        int each = (stages + gridDim.y - 1) / gridDim.y, skip = each * blockIdx.y;
+        stages = max(0, min(each, stages - skip));
+#pragma unroll
+        for (int c = 0; c < COPIES; ++c) from[c] += (int64_t)skip * kStage * pitch[c];
+    }
+    Factors even, odd;
+    auto turn_stage = [&](int k, Factors& f) {
+        if (stages - k >= S)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * COPIES) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (k + S < stages) fetch((k + S) * kStage, lds[now]);
+        now = now + 1 == S ? 0 : now + 1;
+        read(f, lds[now], 0);  // behind the last stage it reads what is there, and nobody uses it
+    };
+#pragma unroll
+    for (int k = 0; k < S; ++k)
+        if (k < stages) fetch(k * kStage, lds[k]);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    read(even, lds[0], 0);
+    if constexpr (STEPS == 2) {
+        for (int k = 0; k < stages; ++k) {
+            read(odd, lds[now], 1);
+            multiply(even);
+            turn_stage(k, even);
+            multiply(odd);
+        }
+    } else if constexpr (P::TILE == 192) {
+        // two sets of factors do not fit in registers beside the sums
+        for (int k = 0; k < stages; ++k) {
+            multiply(even);
+            turn_stage(k, even);
+        }
+    } else {
+        for (int k = 0; k < stages; k += 2) {
+            turn_stage(k, odd);
+            multiply(even);
+            if (k + 1 == stages) break;
+            turn_stage(k + 1, even);
+            multiply(odd);
+        }
+    }
+
+    if (kind == SYMMETRIC && gridDim.y > 1) {
+        // a part of the depth: the sums themselves, a quad of a lane side by side with its neighbours'
+        float4v* to_part = (float4v*)partial + (((int64_t)blockIdx.z * gridDim.x + t) * gridDim.y + blockIdx.y) *
+                                                   (TILE * TILE / 4) + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < SI; ++i)
+#pragma unroll
+            for (int j = 0; j < SJ; ++j)
+#pragma unroll
+                for (int q = 0; q < M::QUADS; ++q) {
+                    float4v v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][q * 4 + e];
+                    to_part[((i * SJ + j) * M::QUADS + q) * P::THREADS] = v;
+                }
+        return;
+    }
+    finish<P, kind, PA>(sums, bi, bj, batch, ep, x, out, to);
+}
+
+// Adds the parts of a symmetric product's tiles up, in their order.
+template <typename P>
+__global__ void __launch_bounds__(P::THREADS) join_kernel(
+    const float* __restrict__ partial, int parts, Epilogue ep, Split x, Split out, int matrices, Split second_out
+) {
+    typedef Mfma<P::SIDE> M;
+    int64_t batch = blockIdx.z;
+    if ((int)blockIdx.z >= matrices) {
+        batch -= matrices;
+        out = second_out;
+    }
+    int bi, bj;
+    triangle(blockIdx.x, bi, bj);
+    Sums<P> sums;
+    const float4v* from = (const float4v*)partial +
+                          ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * parts * (P::TILE * P::TILE / 4) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < Sums<P>::SI; ++i)
+#pragma unroll
+        for (int j = 0; j < Sums<P>::SJ; ++j)
+#pragma unroll
+            for (int q = 0; q < M::QUADS; ++q) {
+                float4v v = (float4v)(0.f);
+                for (int s = 0; s < parts; ++s)
+                    v += from[(int64_t)s * (P::TILE * P::TILE / 4) + ((i * Sums<P>::SJ + j) * M::QUADS + q) * P::THREADS];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sums.acc[i][j][q * 4 + e] = v[e];
+            }
+    finish<P, SYMMETRIC, 2>(sums, bi, bj, batch, ep, x, out, Target{});
 }
 
 // ------------------------------------------------------------------------------------------------ small matrices
@@ -686,23 +770,33 @@ int64_t tiles_of(int64_t m, int64_t n, int64_t batch, bool lower, int64_t side) 
     return (lower ? r * (r + 1) / 2 : r * c) * batch;
 }
 
-// The tile side for the results of m x n (of which the lower triangle, or all): the one whose busiest compute unit is
-// done first. Clocks of a stage of two planes, measured: of a tile that has its compute unit to itself, and of one among
-// those that share it. Small tiles fill the chip where there are few; large ones need less from memory a product.
-int side_of(int64_t m, int64_t n, int64_t batch, bool lower) {
+// How a product of m x n results (of which the lower triangle, or all) is cut: the tile side, and the parts of its depth.
+// Taken is what has the busiest compute unit done first. Clocks of a stage of two planes, measured: of a tile that has
+// its compute unit to itself, and of one among those that share it. Small tiles fill the chip where there are few; large
+// ones need less from memory a product. Parts cost their sums' way through memory and another launch.
+struct Plan {
+    int side, parts;
+};
+
+Plan plan_of(int64_t m, int64_t n, int64_t depth, int64_t batch, bool lower) {
     static const struct { int side; double alone, shared; } costs[] = {
         {256, 5650, 5650}, {192, 4200, 4200}, {128, 2260, 1730}, {96, 1650, 1190}, {64, 900, 640}
     };
-    int best = 0;
+    Plan best{0, 1};
     double least = 0;
-    for (const auto& k : costs) {
-        int64_t each = (tiles_of(m, n, batch, lower, k.side) + 255) / 256;
-        double time = std::max(k.alone, each * k.shared);
-        if (!best || time < least) {
-            least = time;
-            best = k.side;
+    int64_t stages = up(depth, kStage) / kStage;
+    for (const auto& k : costs)
+        for (int64_t parts = 1; parts <= (lower ? stages / 16 : 1) || parts == 1; ++parts) {
+            if (parts > 64) break;
+            int64_t tiles = tiles_of(m, n, batch, lower, k.side) * parts, each = (tiles + 255) / 256;
+            double clocks = std::max(k.alone, each * k.shared) * ((stages + parts - 1) / parts);
+            // 2300 clocks a microsecond; 4 us for the launch, and 4 bytes of a sum there and back at 4 TB/s
+            if (parts > 1) clocks += 2300 * (4 + tiles * k.side * k.side * 8 / 4e6);
+            if (!best.side || clocks < least) {
+                least = clocks;
+                best = {k.side, (int)parts};
+            }
         }
-    }
     return best;
 }
 
@@ -739,9 +833,11 @@ torch::Tensor newton_schulz(
     TORCH_CHECK(steps >= 1 && batch < 32768 && n <= (1 << 20) && scales.size() == 5,
                 "orthogonalize: at least one step, fewer than 32768 matrices and sides of up to 2^20");
     double sx = scales[0], sg = scales[1], sb = scales[2], sq = scales[3], sp = scales[4];
-    int lower = side_of(m, m, batch, true), both = side_of(m, m, 2 * batch, true), rect = side_of(m, n, batch, false);
+    Plan gram_plan = plan_of(m, m, n, batch, true), one_plan = plan_of(m, m, m, batch, true),
+         two_plan = plan_of(m, m, m, 2 * batch, true);
+    int rect = plan_of(m, n, m, batch, false).side;
     // rows that tiles of either side reach, and whole tiles of the packing kernel
-    int64_t mp = std::max({up(m, lower), up(m, both), up(m, rect), up(m, kEdge)}), np = std::max(up(n, rect), up(n, kEdge));
+    int64_t mp = std::max({up(m, gram_plan.side), up(m, one_plan.side), up(m, two_plan.side), up(m, rect), up(m, kEdge)}), np = std::max(up(n, rect), up(n, kEdge));
     int depth_m = (int)up(m, kStage), depth_n = (int)up(n, kStage);
     Matrix in{matrices.data_ptr(), matrices.stride(0), matrices.stride(tall ? 2 : 1), matrices.stride(tall ? 1 : 2),
               (int)m, (int)n};
@@ -784,23 +880,34 @@ torch::Tensor newton_schulz(
                                                       rest.data_ptr<float>());
         HIP_CHECK_LAST();
     });
+    int64_t most = 0;
+    for (const auto& [plan, count] : {std::pair(gram_plan, batch), std::pair(one_plan, batch), std::pair(two_plan, 2 * batch)})
+        if (plan.parts > 1)
+            most = std::max(most, tiles_of(m, m, count, true, plan.side) * plan.parts * plan.side * plan.side);
+    auto sums = torch::empty({most}, matrices.options().dtype(torch::kFloat32));
+    float* partial_sums = sums.data_ptr<float>();
     // out = (alpha A B^T + beta E) scaled, for symmetric results; with a second B and out if given
     auto symmetric = [&](Split u, Split v, int depth, Epilogue ep, Split e, Split out, bool single,
                          const Split* v2 = nullptr, const Split* out2 = nullptr) {
         int64_t count = v2 ? 2 * batch : batch;
-        int side = side_of(m, m, count, true);
-        by_side(side, tiles_of(m, m, count, true, side), [&](auto shape) {
+        Plan plan = v2 ? two_plan : depth == depth_m ? one_plan : gram_plan;
+        by_side(plan.side, tiles_of(m, m, count, true, plan.side) * plan.parts, [&](auto shape) {
             using P = decltype(shape);
-            unsigned r = (unsigned)up(m, P::TILE) / P::TILE;
-            dim3 grid(r * (r + 1) / 2, 1, (unsigned)count);
+            unsigned r = (unsigned)up(m, P::TILE) / P::TILE, tiles = r * (r + 1) / 2;
+            dim3 grid(tiles, (unsigned)plan.parts, (unsigned)count);
             auto go = [&](auto kernel) {
                 kernel<<<grid, P::THREADS, 0, stream>>>(u, v, depth, ep, e, out, to, (int)batch, v2 ? *v2 : v,
-                                                        out2 ? *out2 : out);
+                                                        out2 ? *out2 : out, partial_sums);
             };
             if (single)
                 go(product_kernel<P, SYMMETRIC, 1, 1>);
             else
                 go(product_kernel<P, SYMMETRIC, 2, 2>);
+            if (plan.parts > 1) {
+                HIP_CHECK_LAST();
+                join_kernel<P><<<dim3(tiles, 1, (unsigned)count), P::THREADS, 0, stream>>>(
+                    partial_sums, plan.parts, ep, e, out, (int)batch, out2 ? *out2 : out);
+            }
         });
         HIP_CHECK_LAST();
     };
@@ -812,7 +919,7 @@ torch::Tensor newton_schulz(
             using P = decltype(shape);
             dim3 grid((unsigned)up(n, P::TILE) / P::TILE, (unsigned)up(m, P::TILE) / P::TILE, (unsigned)batch);
             auto go = [&](auto kernel) {
-                kernel<<<grid, P::THREADS, 0, stream>>>(xt, p, depth_m, ep, x, next, to, (int)batch, p, next);
+                kernel<<<grid, P::THREADS, 0, stream>>>(xt, p, depth_m, ep, x, next, to, (int)batch, p, next, nullptr);
             };
             if (last)
                 one ? go(product_kernel<P, LAST, 1, 2>) : go(product_kernel<P, LAST, 2, 2>);

@@ -204,6 +204,13 @@ def test_gpu_steps(shape, steps, coefficients):
 
 
 @gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('shape', [(40, 3000), (130, 8000), (7000, 33), (2, 190, 2500), (1100, 1500)])
+def test_gpu_depth_in_parts(shape, dtype):
+    check(case(*shape, dtype=dtype, device='cuda'))
+
+
+@gpu
 @pytest.mark.parametrize('shape', [(3, 70, 150), (2, 300, 140)])
 def test_gpu_strides(shape):
     b, m, n = shape
