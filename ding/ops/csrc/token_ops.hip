@@ -85,11 +85,12 @@ __device__ inline float value_in(unsigned long long order) {
     return __int_as_float(bits ^ ((bits >> 31) & 0x7fffffff));
 }
 
-// (x - m) k in one operation, where m k does not overflow; rows at the end of the type's range take two
+// (x - m) k in one operation where m k is small: its rounding, up to 2^-24 of it, is a factor of all sums that cancels in
+// what comes out, but must not leave their range. Rows of huge logits take two operations.
 struct Distance {
     float m, k, mk;
     bool far;
-    __device__ inline Distance(float m_, float k_) : m(m_), k(k_), mk(m_ * k_), far(!(fabsf(m_) < 1e30f && fabsf(mk) < 1e37f)) {}
+    __device__ inline Distance(float m_, float k_) : m(m_), k(k_), mk(m_ * k_), far(!(fabsf(mk) < 1e4f)) {}
     __device__ inline float operator()(float x) const { return far ? (x - m) * k : fmaf(x, k, -mk); }
     template <bool FAR> __device__ inline float at(float x) const { return FAR ? (x - m) * k : fmaf(x, k, -mk); }
     // from one reference to another, both as they are rounded

@@ -9,7 +9,6 @@ backward pass instead of [B,S,V] intermediates.
 from collections import namedtuple
 from typing import Optional
 
-import math
 import torch
 from torch import Tensor
 
@@ -68,7 +67,7 @@ def token_log_prob(
         - logits (:obj:`torch.Tensor`): [..., V] of float32, bfloat16 or float16, of any strides; only a last \
             dimension that is not dense costs a copy. Entries of ``-inf`` are masked tokens.
         - index (:obj:`torch.Tensor`): [...] of integers, the tokens that were taken.
-        - temperature (:obj:`float`): The logits are divided by it. It is positive.
+        - temperature (:obj:`float`): The logits are divided by it; in [1e-30, 1e30].
         - ignore_index (:obj:`Optional[int]`): Rows whose token is this (prompts, padding) are not read: their \
             outputs are 0, their top indexes -1, their gradient 0.
         - entropy (:obj:`bool`): Whether to return the entropy.
@@ -90,8 +89,8 @@ def token_log_prob(
         raise TypeError(f"logits must be floating point and index integers, got {logits.dtype} and {index.dtype}")
     if index.device != logits.device:
         raise ValueError(f"index is on {index.device}, logits on {logits.device}")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-30 <= temperature <= 1e30:  # beyond, its inverse leaves the range of 32 bits
+        raise ValueError(f"temperature must be in [1e-30, 1e30], got {temperature}")
     if not 0 <= top_k <= logits.shape[-1]:
         raise ValueError(f"top_k must be in [0, {logits.shape[-1]}], got {top_k}")
     from ding.ops import dispatch

@@ -244,6 +244,24 @@ def test_gpu_reset_hides_what_was_before():
 
 
 @gpu
+@pytest.mark.parametrize('T', [1, 200])
+def test_gpu_without_gradient(T):
+    x, f, h0, reset = case(T, 2, 30, device='cuda')
+    want = gated_linear_recurrence(x, f, h0, reset)
+    with torch.inference_mode():
+        again = gated_linear_recurrence(x, f, h0, reset)
+    with torch.no_grad():
+        out = gated_linear_recurrence(x.requires_grad_(), f, h0, reset)
+    assert not out[0].requires_grad
+    for a, b, c in zip(want, out, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    h, last = gated_linear_recurrence(x, f, h0.requires_grad_(), reset)
+    assert h.requires_grad and last.requires_grad
+    dx, dh0 = torch.autograd.grad(h.sum(), [x, h0])  # the gates take none
+    assert torch.isfinite(dx).all() and torch.isfinite(dh0).all()
+
+
+@gpu
 def test_gpu_refusals():
     x, f, h0, reset = case(4, 2, 3, device='cuda')
     with pytest.raises(TypeError):

@@ -168,6 +168,8 @@ def test_refusals():
     with pytest.raises(ValueError):
         token_log_prob(logits, index, temperature=float('nan'))
     with pytest.raises(ValueError):
+        token_log_prob(logits, index, temperature=1e-40)
+    with pytest.raises(ValueError):
         token_log_prob(logits, index, top_k=8)
     with pytest.raises(ValueError):
         token_log_prob(logits, index, top_k=-1)
@@ -342,6 +344,39 @@ def test_gpu_only_one_gradient_is_given():
         want, tol = oracle(logits, index, 1.0, None, 3, g if pick == 'log_prob' else None,
                            g if pick == 'entropy' else None, torch.ones(4, 3) if pick == 'top_log_prob' else None)
         close(grad, want['grad'], tol['grad'], pick)
+
+
+@gpu
+@pytest.mark.parametrize('V', [18, 300, 9001])
+def test_gpu_temperatures(V):
+    logits, index = case((4, ), V, torch.float32, 'cuda')
+    for temperature in (1e-30, 1e-3, 1e3, 1e30):
+        got = token_log_prob(logits, index, temperature, entropy=True)
+        want, tol = oracle(logits, index, temperature)
+        close(got.log_prob, want['log_prob'], tol['log_prob'], 'log_prob')
+        close(got.entropy, want['entropy'], tol['entropy'], 'entropy')
+
+
+@gpu
+def test_gpu_without_gradient():
+    logits, index = case((3, 5), 700, torch.bfloat16, 'cuda')
+    want = token_log_prob(logits, index, entropy=True, top_k=2)
+    leaf = logits.detach().requires_grad_()
+    with torch.no_grad():
+        out = token_log_prob(leaf, index, entropy=True, top_k=2)
+    assert not out.log_prob.requires_grad
+    with torch.inference_mode():
+        again = token_log_prob(logits, index, entropy=True, top_k=2)
+    for a, b, c in zip(want, out, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    out = token_log_prob(leaf, index, entropy=True, top_k=2)
+    assert out.log_prob.requires_grad and out.entropy.requires_grad and not out.top_index.requires_grad
+    leaf.data.add_(0)
+    kept = token_log_prob(leaf, index)
+    with torch.no_grad():
+        leaf.add_(1.0)  # what the backward pass reads was changed
+    with pytest.raises(RuntimeError):
+        kept.log_prob.sum().backward()
 
 
 @gpu
