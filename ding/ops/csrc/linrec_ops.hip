@@ -8,9 +8,8 @@
 // Bound by memory: two values read and one written a step forward, three read and two written backward. 32768 steps of
 // 2 x 2048 in bfloat16 take 187 us forward (4.3 TB/s of what has to move; a large copy reaches 4.9) and 358 us backward
 // (3.7 TB/s); waiting for earlier tiles is a tenth of that. Odd numbers of channels cost half as much again: every other
-// row starts between two 4-byte words. The state is
-// 32 bit throughout; the states that the backward pass needs are computed again from starting states kept every
-// kChunk steps, not read from the rounded outputs.
+// row starts between two 4-byte words. The state is 32 bit throughout; the states that the backward pass needs are
+// computed again from the states at the tiles' starts, not read from the rounded outputs.
 //
 // A tile is up to 128 steps of 64 lanes' columns (4 bytes of channels a lane: two of 16 bits, one of 32), held in
 // registers: each of up to 8 waves takes kSteps steps, scans them from nothing, and gives the pair (A, B) that its steps

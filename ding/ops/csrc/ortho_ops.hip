@@ -31,7 +31,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kNormBlocks = 256;  // at most, for one matrix
+constexpr int kNormBlocks = 1024;  // at most, for one matrix
 constexpr int kStage = 32;       // depth of a stage
 constexpr int kEdge = 64;        // tile side of the packing kernel
 
@@ -72,33 +72,38 @@ __device__ inline void split(float v, _Float16& hi, _Float16& lo) {
     lo = (_Float16)(v - (float)hi);
 }
 
-// Sums of squares in 64 bits, where no square of a 32-bit number overflows or vanishes. A workgroup takes lines of the
-// dense direction, 16 bytes a thread where `wide` says that lines start at such an address.
+// Sums of squares in 64 bits, where no square of a 32-bit number overflows or vanishes. Lines of the dense direction are
+// read 16 bytes a thread, four such on their way at a time; they may start at any element.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_kernel(Matrix m, double* __restrict__ partial, int wide) {
-    constexpr int N = 16 / sizeof(T);
+__global__ void __launch_bounds__(kThreads) norm_kernel(Matrix m, double* __restrict__ partial) {
+    constexpr int N = 16 / sizeof(T), AHEAD = 4;
     const T* p = (const T*)m.base + blockIdx.y * m.batch_stride;
     double sum = 0;
     bool flip = m.row_stride < m.col_stride;
     int lines = flip ? m.cols : m.rows, length = flip ? m.rows : m.cols;
     int64_t si = flip ? m.row_stride : m.col_stride, so = flip ? m.col_stride : m.row_stride;
-    int per = wide ? N : 1, groups = (length + per - 1) / per;
-    int64_t n = (int64_t)lines * groups;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) {
-        int64_t line = n < (int64_t)1 << 31 ? (unsigned)i / (unsigned)groups : i / groups;
-        int at = (int)(i - line * groups) * per;
-        const T* q = p + line * so + at * si;
-        if (wide && at + N <= length) {
-            T v[N];
-            __builtin_memcpy(v, q, 16);
+    bool dense = si == 1;
+    int groups = (length + N - 1) / N;
+    int64_t n = (int64_t)lines * groups, stride = (int64_t)gridDim.x * kThreads;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += stride * AHEAD) {
+        T v[AHEAD][N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) sum += (double)to_f(v[e]) * to_f(v[e]);
-        } else {
-            for (int e = 0; e < per && at + e < length; ++e) {
-                double v = to_f(q[e * si]);
-                sum += v * v;
+        for (int k = 0; k < AHEAD; ++k) {
+            int64_t g = i + k * stride;
+            int64_t line = n < (int64_t)1 << 31 ? (unsigned)g / (unsigned)groups : g / groups;
+            int at = (int)(g - line * groups) * N;
+            const T* q = p + line * so + at * si;
+            if (dense && g < n && at + N <= length) {
+                __builtin_memcpy(v[k], q, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[k][e] = g < n && at + e < length ? q[e * si] : from_f<T>(0.f);
             }
         }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum += (double)to_f(v[k][e]) * to_f(v[k][e]);
     }
     __shared__ double part[kThreads / kWave];
     for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
@@ -120,7 +125,8 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(
     __shared__ float tile[kEdge][kEdge + 1];
     __shared__ double sum_s[kThreads / kWave];
     int b = blockIdx.z;
-    double sum = threadIdx.x < parts ? partial[b * parts + threadIdx.x] : 0;
+    double sum = 0;
+    for (int i = threadIdx.x; i < parts; i += kThreads) sum += partial[b * parts + i];
     for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
     if (threadIdx.x % kWave == 0) sum_s[threadIdx.x / kWave] = sum;
     __syncthreads();
@@ -855,7 +861,7 @@ torch::Tensor newton_schulz(
     HIP_CHECK_LAST();
     if (done) return result;
     auto half = matrices.options().dtype(torch::kFloat16);
-    int parts = (int)std::min<int64_t>(kNormBlocks, std::max<int64_t>(1, m * n / (kThreads * 16)));
+    int parts = (int)std::min<int64_t>(kNormBlocks, std::max<int64_t>(1, m * n / (kThreads * 32)));
     auto partial = torch::empty({batch * parts}, matrices.options().dtype(torch::kFloat64));
     auto rest = torch::empty({batch}, matrices.options().dtype(torch::kFloat32));
     std::vector<torch::Tensor> kept;
@@ -868,10 +874,7 @@ torch::Tensor newton_schulz(
     Split x = planes(mp, np), xt = planes(np, mp), g = planes(mp, mp), q = planes(mp, mp);
     by_type(matrices, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
-        int64_t dense = std::min(in.row_stride, in.col_stride), line = std::max(in.row_stride, in.col_stride);
-        int wide = dense == 1 && (line * sizeof(T)) % 16 == 0 && (in.batch_stride * sizeof(T)) % 16 == 0 &&
-                   (uintptr_t)in.base % 16 == 0;
-        norm_kernel<T><<<dim3(parts, (unsigned)batch), kThreads, 0, stream>>>(in, partial.data_ptr<double>(), wide);
+        norm_kernel<T><<<dim3(parts, (unsigned)batch), kThreads, 0, stream>>>(in, partial.data_ptr<double>());
         HIP_CHECK_LAST();
         Split px = x, pt = xt;
         if (one) px.lo = pt.lo = nullptr;
