@@ -152,17 +152,29 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(
         tile[i][j] = in ? to_f(p[(i0 + i) * m.row_stride + (j0 + j) * m.col_stride]) * factor : 0.f;
     }
     __syncthreads();
-#pragma unroll 4
-    for (int r = threadIdx.x / kEdge; r < kEdge; r += kThreads / kEdge) {
-        _Float16 hi, lo;
-        split(tile[r][lane], hi, lo);
-        int64_t at = x.at(b, i0 + r, j0 + lane);
-        x.hi[at] = hi;
-        if (x.lo) x.lo[at] = lo;
-        split(tile[lane][r], hi, lo);
-        at = xt.at(b, j0 + r, i0 + lane);
-        xt.hi[at] = hi;
-        if (x.lo) xt.lo[at] = lo;
+    // 16 bytes a thread, 1 KB a wave
+#pragma unroll
+    for (int k = threadIdx.x; k < kEdge * kEdge / 8; k += kThreads) {
+        int piece = k % 4, r = k / 4 % kEdge, c = k / (4 * kEdge) * 32 + piece * 8;
+        half8 hi, lo;
+        auto write = [&](const Split& to, int64_t at) {
+            *(half8*)(to.hi + at) = hi;
+            if (x.lo) *(half8*)(to.lo + at) = lo;
+        };
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 h, l;
+            split(tile[r][c + e], h, l);
+            hi[e] = h, lo[e] = l;
+        }
+        write(x, x.at(b, i0 + r, j0 + c));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 h, l;
+            split(tile[c + e][r], h, l);
+            hi[e] = h, lo[e] = l;
+        }
+        write(xt, xt.at(b, j0 + r, i0 + c));
     }
 }
 
