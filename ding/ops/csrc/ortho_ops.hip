@@ -37,6 +37,7 @@ constexpr int kEdge = 64;        // tile side of the packing kernel
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
@@ -712,14 +713,26 @@ __global__ void __launch_bounds__(512) small_kernel(Matrix m, Target to, Small p
             for (int i = 0; i < S::XI; ++i)
 #pragma unroll
                 for (int j = 0; j < S::J; ++j)
+                {
+                    // neighbouring lanes hold neighbouring columns: the even one writes both of rows 0 and 1, the odd one
+                    // of rows 2 and 3
+                    bool odd = lane & 1;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                    for (int e = 0; e < 2; ++e) {
+                        float mine = odd ? x[q][i][j][2 + e] : x[q][i][j][e], given = odd ? x[q][i][j][e] : x[q][i][j][2 + e];
+                        float other = __int_as_float(
+                            __builtin_amdgcn_update_dpp(0, __float_as_int(given), 0xb1, 0xf, 0xf, true));
+                        half2v hi, lo;
                         _Float16 h, l;
-                        split(x[q][i][j][e], h, l);
-                        int at = small_at(S::PART, row_x(0, i) + e, c0 + j * 16);
-                        lx[at] = h;
-                        lx[S::X_PLANE + at] = l;
+                        split(odd ? other : mine, h, l);
+                        hi[0] = h, lo[0] = l;
+                        split(odd ? mine : other, h, l);
+                        hi[1] = h, lo[1] = l;
+                        int at = small_at(S::PART, row_x(0, i) + e + (odd ? 2 : 0), (c0 & ~1) + j * 16);
+                        *(half2v*)(lx + at) = hi;
+                        *(half2v*)(lx + S::X_PLANE + at) = lo;
                     }
+                }
             __syncthreads();
             float4v got[S::XI][S::J];
 #pragma unroll
