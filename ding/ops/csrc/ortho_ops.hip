@@ -541,8 +541,10 @@ __global__ void __launch_bounds__(P::THREADS) join_kernel(
 // ------------------------------------------------------------------------------------------------ small matrices
 // A matrix of up to 128 x 256 has a workgroup of its own for the whole iteration: X stays in registers in 32 bits, its
 // factors and G's lie in LDS, and nothing is launched or stored between the products, where a launch of its own takes
-// about 5 us a product whatever its size. Up to 256 matrices of 64 x 64 take 15 us, of 128 x 128 56 us (six of them by
-// launches: 95 us). Of 128 x 256 they take 108 us, six of them by launches 104 us, 64 of them 160 us.
+// about 5 us a product whatever its size. Up to 256 matrices of 64 x 64 take 14 us, of 128 x 128 55 us (six of them by
+// launches: 95 us). Up to 256 of 128 x 256 take 92 to 110 us, by launches six take 104 us and 64 160 us. Products, LDS and the
+// vector unit's splitting take about a third of the time each and hardly overlap: two waves a unit wait at the same
+// barriers.
 // X is held as the results of (B X)^T: rows r of X^T in parts of kPart, columns c; a wave has a half of a part's rows
 // and a quarter of the columns. The same place in LDS holds X and X^T in turns, a part at a time.
 struct Small {
@@ -584,10 +586,21 @@ __global__ void __launch_bounds__(512) small_kernel(Matrix m, Target to, Small p
             for (int j = 0; j < S::J; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    int r = row_x(q, i) + e, c = c0 + j * 16;
-                    float v = 0.f;
-                    if (c < m.rows && r < m.cols)
-                        v = to_f(((const T*)m.base)[blockIdx.x * m.batch_stride + c * m.row_stride + r * m.col_stride]);
+                    // all loads go out before the first is waited for
+                    int r = min(row_x(q, i) + e, m.cols - 1), c = min(c0 + j * 16, m.rows - 1);
+                    x[q][i][j][e] =
+                        to_f(((const T*)m.base)[blockIdx.x * m.batch_stride + c * m.row_stride + r * m.col_stride]);
+                }
+#pragma unroll
+    for (int q = 0; q < S::PARTS; ++q)
+#pragma unroll
+        for (int i = 0; i < S::XI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    bool in = row_x(q, i) + e < m.cols && c0 + j * 16 < m.rows;
+                    float v = in ? x[q][i][j][e] : 0.f;
                     x[q][i][j][e] = v;
                     sum += (double)v * v;
                 }
