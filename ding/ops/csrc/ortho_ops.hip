@@ -816,13 +816,13 @@ int64_t tiles_of(int64_t m, int64_t n, int64_t batch, bool lower, int64_t side) 
 
 // How a product of m x n results (of which the lower triangle, or all) is cut: the tile side, and the parts of its depth.
 // Taken is what has the busiest compute unit done first. Clocks of a stage of two planes, measured: of a tile that has
-// its compute unit to itself, and of one among those that share it. Small tiles fill the chip where there are few; large
+// its compute unit to itself, and of one among those that share it; a single plane takes 0.4 of them. Small tiles fill the chip where there are few; large
 // ones need less from memory a product. Parts cost their sums' way through memory and another launch.
 struct Plan {
     int side, parts;
 };
 
-Plan plan_of(int64_t m, int64_t n, int64_t depth, int64_t batch, bool lower) {
+Plan plan_of(int64_t m, int64_t n, int64_t depth, int64_t batch, bool lower, bool single = false) {
     static const struct { int side; double alone, shared; } costs[] = {
         {256, 5650, 5650}, {192, 4200, 4200}, {128, 2260, 1730}, {96, 1650, 1190}, {64, 900, 640}
     };
@@ -833,7 +833,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t depth, int64_t batch, bool lower) {
         for (int64_t parts = 1; parts <= (lower ? stages / 16 : 1) || parts == 1; ++parts) {
             if (parts > 64) break;
             int64_t tiles = tiles_of(m, n, batch, lower, k.side) * parts, each = (tiles + 255) / 256;
-            double clocks = std::max(k.alone, each * k.shared) * ((stages + parts - 1) / parts);
+            double clocks = std::max(k.alone, each * k.shared) * ((stages + parts - 1) / parts) * (single ? 0.4 : 1.0);
             // 2300 clocks a microsecond; 4 us for the launch, and 4 bytes of a sum there and back at 4 TB/s
             if (parts > 1) clocks += 2300 * (4 + tiles * k.side * k.side * 8 / 4e6);
             if (!best.side || clocks < least) {
@@ -877,11 +877,12 @@ torch::Tensor newton_schulz(
     TORCH_CHECK(steps >= 1 && batch < 32768 && n <= (1 << 20) && scales.size() == 5,
                 "orthogonalize: at least one step, fewer than 32768 matrices and sides of up to 2^20");
     double sx = scales[0], sg = scales[1], sb = scales[2], sq = scales[3], sp = scales[4];
-    Plan gram_plan = plan_of(m, m, n, batch, true), one_plan = plan_of(m, m, m, batch, true),
+    bool one = matrices.scalar_type() != torch::kFloat32;  // X has one plane until it is updated
+    Plan first_plan = plan_of(m, m, n, batch, true, one), gram_plan = plan_of(m, m, n, batch, true), one_plan = plan_of(m, m, m, batch, true),
          two_plan = plan_of(m, m, m, 2 * batch, true);
     int rect = plan_of(m, n, m, batch, false).side;
     // rows that tiles of either side reach, and whole tiles of the packing kernel
-    int64_t mp = std::max({up(m, gram_plan.side), up(m, one_plan.side), up(m, two_plan.side), up(m, rect), up(m, kEdge)}), np = std::max(up(n, rect), up(n, kEdge));
+    int64_t mp = std::max({up(m, first_plan.side), up(m, gram_plan.side), up(m, one_plan.side), up(m, two_plan.side), up(m, rect), up(m, kEdge)}), np = std::max(up(n, rect), up(n, kEdge));
     int depth_m = (int)up(m, kStage), depth_n = (int)up(n, kStage);
     Matrix in{matrices.data_ptr(), matrices.stride(0), matrices.stride(tall ? 2 : 1), matrices.stride(tall ? 1 : 2),
               (int)m, (int)n};
@@ -908,7 +909,6 @@ torch::Tensor newton_schulz(
         _Float16* p = (_Float16*)kept.back().data_ptr();
         return Split{p, p + batch * r * q, r * q, (int)r};
     };
-    bool one = type != 0;  // X has one plane until it is updated
     Split x = planes(mp, np), xt = planes(np, mp), g = planes(mp, mp), q = planes(mp, mp);
     by_type(matrices, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
@@ -922,7 +922,7 @@ torch::Tensor newton_schulz(
         HIP_CHECK_LAST();
     });
     int64_t most = 0;
-    for (const auto& [plan, count] : {std::pair(gram_plan, batch), std::pair(one_plan, batch), std::pair(two_plan, 2 * batch)})
+    for (const auto& [plan, count] : {std::pair(first_plan, batch), std::pair(gram_plan, batch), std::pair(one_plan, batch), std::pair(two_plan, 2 * batch)})
         if (plan.parts > 1)
             most = std::max(most, tiles_of(m, m, count, true, plan.side) * plan.parts * plan.side * plan.side);
     auto sums = torch::empty({most}, matrices.options().dtype(torch::kFloat32));
@@ -931,7 +931,7 @@ torch::Tensor newton_schulz(
     auto symmetric = [&](Split u, Split v, int depth, Epilogue ep, Split e, Split out, bool single,
                          const Split* v2 = nullptr, const Split* out2 = nullptr) {
         int64_t count = v2 ? 2 * batch : batch;
-        Plan plan = v2 ? two_plan : depth == depth_m ? one_plan : gram_plan;
+        Plan plan = v2 ? two_plan : single ? first_plan : depth == depth_m ? one_plan : gram_plan;
         by_side(plan.side, tiles_of(m, m, count, true, plan.side) * plan.parts, [&](auto shape) {
             using P = decltype(shape);
             unsigned r = (unsigned)up(m, P::TILE) / P::TILE, tiles = r * (r + 1) / 2;
