@@ -21,6 +21,11 @@
 // taken for results that are rounded to 16 bits, over so many steps that its error stays below a fraction of that
 // rounding (five for bfloat16, three for float16).
 //
+// Large products run at 1.0 to 1.2 PFLOP/s of 16-bit instructions (4096 x 4096 over 8192: 674 us; a library's product of
+// plain half precision reaches 1.3 here, and the instructions alone 1.4 with every unit busy), so a third of that in
+// results; 32-bit library products reach 0.15. What keeps smaller ones lower is LDS, which every tile's factors pass twice, and
+// some 10 us a launch of filling, storing and starting.
+//
 // All products are "row times row" (C_ij = sum_k A_ik B_jk), which needs X and its transpose: both are kept. Columns are
 // padded with zeros to a multiple of a stage's depth; rows of a tile that lie behind them are memory of ours that may
 // hold anything, and reach nothing but such rows of the results.
@@ -878,11 +883,15 @@ torch::Tensor newton_schulz(
                 "orthogonalize: at least one step, fewer than 32768 matrices and sides of up to 2^20");
     double sx = scales[0], sg = scales[1], sb = scales[2], sq = scales[3], sp = scales[4];
     bool one = matrices.scalar_type() != torch::kFloat32;  // X has one plane until it is updated
-    Plan first_plan = plan_of(m, m, n, batch, true, one), gram_plan = plan_of(m, m, n, batch, true), one_plan = plan_of(m, m, m, batch, true),
-         two_plan = plan_of(m, m, m, 2 * batch, true);
+    Plan first_plan = plan_of(m, m, n, batch, true, one), gram_plan = plan_of(m, m, n, batch, true);
+    Plan one_plan = plan_of(m, m, m, batch, true), two_plan = plan_of(m, m, m, 2 * batch, true);
+    const std::pair<Plan, int64_t> plans[] = {
+        {first_plan, batch}, {gram_plan, batch}, {one_plan, batch}, {two_plan, 2 * batch}
+    };
     int rect = plan_of(m, n, m, batch, false).side;
     // rows that tiles of either side reach, and whole tiles of the packing kernel
-    int64_t mp = std::max({up(m, first_plan.side), up(m, gram_plan.side), up(m, one_plan.side), up(m, two_plan.side), up(m, rect), up(m, kEdge)}), np = std::max(up(n, rect), up(n, kEdge));
+    int64_t mp = std::max(up(m, rect), up(m, kEdge)), np = std::max(up(n, rect), up(n, kEdge));
+    for (const auto& [plan, count] : plans) mp = std::max(mp, up(m, plan.side));
     int depth_m = (int)up(m, kStage), depth_n = (int)up(n, kStage);
     Matrix in{matrices.data_ptr(), matrices.stride(0), matrices.stride(tall ? 2 : 1), matrices.stride(tall ? 1 : 2),
               (int)m, (int)n};
@@ -922,7 +931,7 @@ torch::Tensor newton_schulz(
         HIP_CHECK_LAST();
     });
     int64_t most = 0;
-    for (const auto& [plan, count] : {std::pair(first_plan, batch), std::pair(gram_plan, batch), std::pair(one_plan, batch), std::pair(two_plan, 2 * batch)})
+    for (const auto& [plan, count] : plans)
         if (plan.parts > 1)
             most = std::max(most, tiles_of(m, m, count, true, plan.side) * plan.parts * plan.side * plan.side);
     auto sums = torch::empty({most}, matrices.options().dtype(torch::kFloat32));

@@ -9,10 +9,16 @@
 // once. Everything is kept in base 2 relative to the row's maximum: with k = log2(e) / T, d_v = (x_v - max) k,
 // s = sum 2^d, t = sum 2^d d, so log p = ln2 (d - log2 s) and H = ln2 (log2 s - t / s). All sums are 32 bit.
 //
-// A row is cut into equal segments of up to 8192 logits, one workgroup each: every thread holds 32 in registers, so a
-// segment is read once, also where its largest entries are wanted. The segments of a row are joined by a second,
-// small kernel; a row of one segment needs none. Rows of up to 512 entries (action sets) share a workgroup instead,
-// 16 or 64 lanes a row.
+// Four ways over the rows, every thread holding 32 logits in registers, so that logits are read once also where the
+// largest are wanted:
+//   up to 512 entries (action sets): 16 or 64 lanes a row, several rows a workgroup;
+//   up to 256 longer rows: segments of up to 32768 logits, 1024 threads each (32 rows of 32000 bf16 with entropy and the
+//   eight largest: 13 us a call, 18 us in segments of 8192);
+//   from 1024 rows on, where no largest are wanted: a workgroup walks a row of its own, see token_stream_fwd;
+//   else equal segments of up to 8192 logits, 256 threads each.
+// The segments of a row are joined by a second, small kernel; a row of one segment needs none.
+// 16384 rows of 131072 bf16 logits, three quarters of them live, take 0.59 ms forward (5.4 TB/s) and 1.33 ms backward
+// (5.6 TB/s); a large copy reaches 4.9 TB/s here.
 #include "common.h"
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -24,6 +30,7 @@ constexpr int kPerThread = 32;
 constexpr int kSegment = kThreads * kPerThread;
 constexpr int kMostTop = 32;
 constexpr int64_t kManyRows = 1024;
+constexpr int64_t kFewRows = 256;  // one for each compute unit
 constexpr int kMostJoined = 4096;  // candidates that a row's segments may offer
 constexpr float kLn2 = 0.69314718055994531f;
 // 2^-200 is zero in 32 bits: entries that far below the maximum count nothing, and 0 * -inf is kept out of the sums
@@ -252,7 +259,7 @@ __global__ void __launch_bounds__(kThreads) token_short_fwd(
 // `top` largest of n orders in LDS, in descending order: each one's place is the number of larger ones
 template <typename F>
 __device__ inline void rank_orders(const unsigned long long* orders, int n, int top, F&& put) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
         unsigned long long mine = orders[i];
         if (mine == 0) continue;
         int larger = 0;
@@ -261,8 +268,8 @@ __device__ inline void rank_orders(const unsigned long long* orders, int n, int 
     }
 }
 
-template <typename T, bool TOP, bool ENTROPY>
-__global__ void __launch_bounds__(kThreads) token_segment_fwd(
+template <typename T, bool TOP, bool ENTROPY, int THREADS>
+__global__ void __launch_bounds__(THREADS) token_segment_fwd(
     Rows rows, const int64_t* __restrict__ index, Out out, int V, int segments, int length, float k, int64_t ignore,
     int has_ignore, int top, float* __restrict__ partial, unsigned long long* __restrict__ offered
 ) {
@@ -272,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
     int tid = threadIdx.x;
     int64_t token = index[r];
     if (has_ignore && token == ignore) {
-        if (seg == 0) write_nothing(out, r, top, tid, kThreads);
+        if (seg == 0) write_nothing(out, r, top, tid, THREADS);
         return;
     }
     const T* x = row_of<T>(rows, r);
@@ -280,7 +287,7 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
     Pack<T> v[kPerThread / N];
 #pragma unroll
     for (int j = 0; j < kPerThread / N; ++j) {
-        int c = lo + (j * kThreads + tid) * N;
+        int c = lo + (j * THREADS + tid) * N;
         if (c + N <= hi) {
             v[j] = load_pack(x + c);
         } else {
@@ -312,14 +319,15 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
         add(std::false_type{});
     a.s = group_sum<kWave>(a.s);
     if (ENTROPY) a.t = group_sum<kWave>(a.t);
-    __shared__ Sums part[kThreads / kWave];
+    __shared__ Sums part[THREADS / kWave];
     if (tid % kWave == 0) part[tid / kWave] = a;
 
-    // Largest entries. Of the threads' own largest, the top-th is a bound that all wanted entries reach, and only
-    // `top` threads hold entries that reach it: at most top * kPerThread candidates.
-    __shared__ unsigned long long best[TOP ? kThreads : 1];
+    // Largest entries. Of the largest of 64 groups of lanes, the top-th is a bound that all wanted entries reach, and only
+    // `top` groups hold entries that reach it: at most top * GROUP * kPerThread candidates, and far fewer as a rule.
+    constexpr int GROUP = THREADS / 64;
+    __shared__ unsigned long long best[TOP ? 64 : 1];
     __shared__ unsigned long long bound_s;
-    __shared__ unsigned long long candidates[TOP ? kMostTop * kPerThread : 1];
+    __shared__ unsigned long long candidates[TOP ? kMostTop * GROUP * kPerThread : 1];
     __shared__ int found;
     if constexpr (TOP) {
         unsigned long long mine = 0;
@@ -327,26 +335,31 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
         for (int j = 0; j < kPerThread / N; ++j)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                int c = lo + (j * kThreads + tid) * N + i;
+                int c = lo + (j * THREADS + tid) * N + i;
                 unsigned long long o = c < hi ? order_of(to_f(v[j].v[i]), c) : 0;
                 mine = o > mine ? o : mine;
             }
-        best[tid] = mine;
+        mine = group_max<GROUP>(mine);
+        if (tid % GROUP == 0) best[tid / GROUP] = mine;
         if (tid == 0) {
-            bound_s = 1;  // fewer than `top` threads hold entries: all of theirs are candidates
+            bound_s = 1;  // fewer than `top` groups hold entries: all of theirs are candidates
             found = 0;
         }
         __syncthreads();
-        int larger = 0;
-        for (int j = 0; j < kThreads; ++j) larger += best[j] > mine;
-        if (mine != 0 && larger == top - 1) bound_s = mine;
+        if (tid < 64) {
+            mine = best[tid];
+            int larger = 0;
+#pragma unroll 8
+            for (int j = 0; j < 64; ++j) larger += best[j] > mine;
+            if (mine != 0 && larger == top - 1) bound_s = mine;
+        }
         __syncthreads();
         unsigned long long bound = bound_s;
 #pragma unroll
         for (int j = 0; j < kPerThread / N; ++j)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                int c = lo + (j * kThreads + tid) * N + i;
+                int c = lo + (j * THREADS + tid) * N + i;
                 unsigned long long o = c < hi ? order_of(to_f(v[j].v[i]), c) : 0;
                 if (o >= bound) candidates[atomicAdd(&found, 1)] = o;
             }
@@ -354,7 +367,7 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
     __syncthreads();
     Sums all = part[0];
 #pragma unroll
-    for (int w = 1; w < kThreads / kWave; ++w) all = join(all, part[w], k);
+    for (int w = 1; w < THREADS / kWave; ++w) all = join(all, part[w], k);
     if (segments == 1) {
         if (tid == 0) write_row(out, r, all, x, token, V, k);
         if constexpr (TOP) {
@@ -372,7 +385,7 @@ __global__ void __launch_bounds__(kThreads) token_segment_fwd(
         }
         if constexpr (TOP) {
             unsigned long long* mine = offered + (int64_t)blockIdx.x * top;
-            for (int j = tid; j < top; j += kThreads)
+            for (int j = tid; j < top; j += THREADS)
                 if (j >= found) mine[j] = 0;
             rank_orders(candidates, found, top, [&](int j, unsigned long long o) { mine[j] = o; });
         }
@@ -683,9 +696,11 @@ std::vector<torch::Tensor> token_log_prob_fwd(
     Rows rows = rows_of(logits);
     int64_t count = index.numel();
     int V = (int)logits.size(-1);
-    int segments = cdiv(V, kSegment);
+    // few long rows: four times as many threads hold a segment, which saves the joining launch up to 32768 entries
+    bool large = count <= kFewRows && V > kSegment;
+    int segments = cdiv(V, large ? 4 * kSegment : kSegment);
     TORCH_CHECK(top >= 0 && top <= kMostTop && top <= V, "token_log_prob: top_k must be at most ", kMostTop, " and V");
-    TORCH_CHECK(top * segments <= kMostJoined, "token_log_prob: top_k of ", top, " over ", V, " entries is too much");
+    TORCH_CHECK(segments == 1 || top * segments <= kMostJoined, "token_log_prob: top_k of ", top, " over ", V, " entries is too much");
     auto opt = logits.options().dtype(torch::kFloat32);
     auto tops = index.sizes().vec();
     tops.push_back(top);
@@ -730,14 +745,17 @@ std::vector<torch::Tensor> token_log_prob_fwd(
             dim3 grid((unsigned)(count * segments));
             int length = length_of(V, segments);
             auto go = [&](auto kernel) {
-                kernel<<<grid, kThreads, 0, stream>>>(rows, ix, out, V, segments, length, k, ignore, has_ignore, top, p, o);
+                kernel<<<grid, large ? 4 * kThreads : kThreads, 0, stream>>>(rows, ix, out, V, segments, length, k, ignore,
+                                                                              has_ignore, top, p, o);
             };
             if (top > 0)
-                go(token_segment_fwd<T, true, true>);
+                large ? go(token_segment_fwd<T, true, true, 4 * kThreads>) : go(token_segment_fwd<T, true, true, kThreads>);
+            else if (large)
+                go(token_segment_fwd<T, false, true, 4 * kThreads>);
             else if (want_entropy)
-                go(token_segment_fwd<T, false, true>);
+                go(token_segment_fwd<T, false, true, kThreads>);
             else
-                go(token_segment_fwd<T, false, false>);
+                go(token_segment_fwd<T, false, false, kThreads>);
             if (segments > 1) {
                 HIP_CHECK_LAST();
                 if (top > 0)

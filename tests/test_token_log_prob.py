@@ -222,6 +222,27 @@ def test_gpu_top(V, top_k):
 
 
 @gpu
+@pytest.mark.parametrize('rows', [256, 257])
+@pytest.mark.parametrize('V,top_k', [(8200, 1), (20000, 7), (40000, 32)])
+def test_gpu_top_of_many_rows(rows, V, top_k):
+    gen = torch.Generator(device='cuda').manual_seed(V)
+    logits = torch.empty(rows, V, device='cuda').normal_(0, 2, generator=gen).bfloat16()
+    logits[0] = 1.0
+    logits[1] = torch.arange(V, device='cuda').float().div(V).bfloat16()  # long runs of equal logits
+    logits[2] = -torch.arange(V, device='cuda').float().bfloat16()
+    logits[3, 5:] = float('-inf')
+    index = torch.randint(0, V, (rows, ), device='cuda', generator=gen)
+    index[3] = 2
+    got = token_log_prob(logits, index, entropy=True, top_k=top_k)
+    want = torch.sort(logits.float(), dim=-1, descending=True, stable=True).indices[:, :top_k]
+    assert torch.equal(got.top_index, want)
+    keep = list(range(6)) + [100, rows - 1]
+    want, tol = oracle(logits[keep], index[keep], 1.0, None, top_k)
+    close(got.top_log_prob[keep], want['top_log_prob'], tol['top_log_prob'], 'top_log_prob')
+    close(got.entropy[keep], want['entropy'], tol['entropy'], 'entropy')
+
+
+@gpu
 @pytest.mark.parametrize('V', [30, 300, 1025, 9001])
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 def test_gpu_masks(V, dtype):
