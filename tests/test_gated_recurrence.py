@@ -354,3 +354,38 @@ def test_gpu_module():
     assert torch.allclose(want, got.cpu(), atol=1e-4) and state[0]['h'].is_cuda
     got.sum().backward()
     assert all(torch.isfinite(p.grad).all() for p in rnn.parameters())
+
+
+def _r2d2(cuda):
+    from ding.policy import create_policy
+    from ding.policy.base_policy import get_policy_cls
+    from ding.utils import EasyDict, deep_merge_dicts
+    cfg = dict(
+        type='r2d2', cuda=cuda, on_policy=False,
+        model=dict(obs_shape=8, action_shape=3, encoder_hidden_size_list=[32, 32], lstm_type='glr'),
+        learn=dict(batch_size=4), collect=dict(unroll_len=8, env_num=2), unroll_len=8, nstep=2, burnin_step=2,
+    )
+    cfg = EasyDict(deep_merge_dicts(get_policy_cls(EasyDict(dict(type='r2d2'))).default_config(), cfg))
+    policy = create_policy(cfg, enable_field=['learn', 'collect'])
+    gen = torch.Generator().manual_seed(0)
+    samples = [{
+        'obs': [torch.randn(8, generator=gen) for _ in range(8)],
+        'action': [torch.randint(0, 3, (), generator=gen) for _ in range(8)],
+        'reward': [torch.randn(2, generator=gen) for _ in range(8)],
+        'done': [False] * 8,
+        'prev_state': [None] * 8,
+    } for _ in range(4)]
+    info = policy._forward_learn(samples)
+    assert torch.isfinite(torch.as_tensor(float(info['total_loss'])))
+    for _ in range(2):  # a collector's steps, with the states that the first left
+        out = policy._forward_collect({i: torch.randn(8, generator=gen) for i in range(2)}, eps=0.1)
+        assert set(out) == {0, 1}
+
+
+def test_recurrent_policy_cpu():
+    _r2d2(False)
+
+
+@gpu
+def test_recurrent_policy_gpu():
+    _r2d2(True)
