@@ -394,6 +394,10 @@ __global__ void __launch_bounds__(kMostWaves* kWave, 4) linrec_bwd_kernel(
         }
     __shared__ float la[kMostWaves][kWave * N], lb[kMostWaves][kWave * N], lq[kMostWaves][kWave * N];
     __shared__ Window<N> window;
+    // the gradients wait in LDS for the last pass: with them the registers of two workgroups a compute unit do not do
+    __shared__ uint32_t waiting[STEPS][kMostWaves * kWave];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) waiting[i][threadIdx.x] = rg[i];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         la[wave][lane * N + j] = A[j];
@@ -457,10 +461,11 @@ __global__ void __launch_bounds__(kMostWaves* kWave, 4) linrec_bwd_kernel(
 #pragma unroll
     for (int i = STEPS - 1; i >= 0; --i) {
         float vx[2], vf[2];
+        uint32_t raw = waiting[i][threadIdx.x];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             asm volatile("" : "+v"(e[i][j]));
-            float a, b, G = m[j] + value_of(rg[i], j, (T*)nullptr);
+            float a, b, G = m[j] + value_of(raw, j, (T*)nullptr);
             gate(e[i][j], a, b);
             vx[j] = b * G;
             vf[j] = G * apart[i][j] * a * b;
