@@ -324,7 +324,8 @@ def orthogonalize(
         products run on the matrix units to 22 bits (HIP kernels, ding/ops/csrc/ortho_ops.hip). Not differentiable.
     Arguments:
         - matrix (:obj:`torch.Tensor`): [..., m, n] of float32, bfloat16 or float16, any strides; a batch is \
-            orthogonalised together, which is faster than one matrix after the other.
+            orthogonalised together, which is faster than one matrix after the other. On a GPU sides are at most \
+            2^20 and matrices fewer than 32768.
         - steps (:obj:`int`): Number of steps, at least 1.
         - coefficients (:obj:`Tuple[float, float, float]`): a, b and c.
         - eps (:obj:`float`): Is added to the norm: a zero matrix gives zeros. On a GPU entries are held to about \
@@ -458,8 +459,11 @@ class Muon(torch.optim.Optimizer):
         torch._foreach_mul_(bufs, group['momentum'])
         torch._foreach_add_(bufs, grads)
         updates = torch._foreach_add(grads, bufs, alpha=group['momentum']) if group['nesterov'] else bufs
-        # in the weights' type: the step is rounded to it when it is added to them anyway
-        stacked = torch.stack([u.reshape(shape) for u in updates]).to(params[0].dtype)
+        # In the weights' type: the step is rounded to it when it is added to them anyway. Not in half precision, whose
+        # range a sum of gradients passes.
+        dtype = params[0].dtype
+        stacked = torch.stack([u.reshape(shape) for u in updates])
+        stacked = stacked if dtype == torch.float16 else stacked.to(dtype)
         update = orthogonalize(stacked, group['ns_steps'], group['ns_coefficients'], group['ns_eps'])
         step = group['lr'] * 0.2 * math.sqrt(max(shape))
         torch._foreach_add_(params, [u.view(p.shape) for u, p in zip(update.unbind(0), params)], alpha=-step)

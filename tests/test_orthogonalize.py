@@ -159,6 +159,28 @@ def test_optimizer_cpu():
     _check_optimizer('cpu', torch.float32, 4 * 0.012 * 1e-4 + 8 * 2.0 ** -24)
 
 
+def _check_half_weights(device):
+    """Weights of half precision whose gradients are near either end of its range: their momentum passes it."""
+    for size in (60000.0, 2.0 ** -22):
+        torch.manual_seed(3)
+        net = torch.nn.Conv2d(6, 20, 3, bias=False).to(device=device, dtype=torch.float16)
+        net = net.to(memory_format=torch.channels_last)
+        p, opt, grads = net.weight, Muon(net.parameters(), lr=0.01), []
+        start = p.detach().clone()
+        for step in range(4):
+            sign = torch.randint(0, 2, p.shape, generator=torch.Generator().manual_seed(step // 3)) * 2 - 1
+            p.grad = (sign * size).to(device=device, dtype=torch.float16)
+            grads.append(p.grad.clone())
+            opt.step()
+        want = _want_step(start, grads, opt.param_groups[0])
+        # a rounding of the weight a step, and steps of 0.01 * 0.2 sqrt(54) times updates that are right to 1e-4
+        assert (p.detach().cpu().double() - want).abs().max() <= 4 * 2.0 ** -11 * want.abs().max() + 4 * 0.015 * 1e-4
+
+
+def test_optimizer_half_weights_cpu():
+    _check_half_weights('cpu')
+
+
 def test_optimizer_options():
     net = _net()
     for clip in (dict(grad_clip_type='clip_norm', clip_value=0.5), dict(grad_clip_type='clip_value', clip_value=0.1),
@@ -272,6 +294,11 @@ def test_gpu_stream_and_graph():
 @gpu
 def test_gpu_optimizer():
     _check_optimizer('cuda', torch.float32, 4 * 0.012 * 1e-4 + 8 * 2.0 ** -24)
+
+
+@gpu
+def test_gpu_optimizer_half_weights():
+    _check_half_weights('cuda')
 
 
 @gpu
