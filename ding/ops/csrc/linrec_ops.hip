@@ -6,9 +6,9 @@
 //   G_t = g_t + r_{t+1} a_{t+1} G_{t+1}   (g_last joins at the last step)
 //   dx_t = (1 - a_t) G_t,  df_t = G_t (r_t h_{t-1} - x_t) a_t (1 - a_t),  dh0 = r_0 a_0 G_0
 // Bound by memory: two values read and one written a step forward, three read and two written backward. 32768 steps of
-// 2 x 2048 in bfloat16 take 187 us forward (4.3 TB/s of what has to move; a large copy reaches 4.9) and 358 us backward
-// (3.7 TB/s); waiting for earlier tiles is a tenth of that. Odd numbers of channels cost half as much again: every other
-// row starts between two 4-byte words. The state is 32 bit throughout; the states that the backward pass needs are
+// 2 x 2048 in bfloat16 take 187 us forward (4.3 TB/s of what has to move; a large copy reaches 4.9) and 292 us backward
+// (4.6 TB/s); waiting for earlier tiles is a tenth of that. Odd numbers of 16-bit channels cost a quarter more: every
+// other row starts between two 4-byte words. The state is 32 bit throughout; the states that the backward pass needs are
 // computed again from the states at the tiles' starts, not read from the rounded outputs.
 //
 // A tile is up to 128 steps of 64 lanes' columns (4 bytes of channels a lane: two of 16 bits, one of 32), held in

@@ -172,21 +172,25 @@ struct Out {
 
 __device__ inline float log2_of(float s) { return __builtin_amdgcn_logf(s); }
 
+// What roundings put on the wrong side of zero is zero; NaN stays.
+__device__ inline float at_most_zero(float v) { return v > 0.f ? 0.f : v; }
+__device__ inline float at_least_zero(float v) { return v < 0.f ? 0.f : v; }
+
 // what one lane writes for a row whose sums are known
 template <typename T>
 __device__ inline void write_row(const Out& out, int64_t r, Sums a, const T* x, int64_t token, int V, float k) {
     float log2s = log2_of(a.s);
     float lp = __builtin_nanf("");
-    if (token >= 0 && token < V) lp = (Distance(a.m, k)(to_f(x[token])) - log2s) * kLn2;
+    if (token >= 0 && token < V) lp = at_most_zero((Distance(a.m, k)(to_f(x[token])) - log2s) * kLn2);
     out.log_prob[r] = lp;
-    if (out.entropy) out.entropy[r] = (log2s - a.t / a.s) * kLn2;
+    if (out.entropy) out.entropy[r] = at_least_zero((log2s - a.t / a.s) * kLn2);
     out.stats[2 * r] = a.m;
     out.stats[2 * r + 1] = log2s;
 }
 
 __device__ inline void write_top(const Out& out, int64_t r, int top, int j, unsigned long long order, float m,
                                  float log2s, float k) {
-    out.top_log_prob[r * top + j] = (Distance(m, k)(value_in(order)) - log2s) * kLn2;
+    out.top_log_prob[r * top + j] = at_most_zero((Distance(m, k)(value_in(order)) - log2s) * kLn2);
     out.top_index[r * top + j] = index_in(order);
 }
 

@@ -368,6 +368,24 @@ def test_gpu_only_one_gradient_is_given():
 
 
 @gpu
+@pytest.mark.parametrize('rows', [8, 1100])
+@pytest.mark.parametrize('V', [1, 2, 18, 500, 5000, 40000])
+def test_gpu_signs(rows, V):
+    """Rows of one likely token: no rounding makes a probability larger than 1 or an entropy negative."""
+    gen = torch.Generator().manual_seed(V)
+    logits = torch.randn(rows, V, generator=gen).cuda()
+    index = torch.randint(0, V, (rows,), generator=gen).cuda()
+    logits[torch.arange(rows).cuda(), index] = torch.logspace(0, 4, rows).cuda()
+    for top in (0, min(V, 2)):
+        out = token_log_prob(logits, index, temperature=0.7, entropy=True, top_k=top)
+        assert (out.log_prob <= 0).all() and (out.entropy >= 0).all()
+        assert top == 0 or (out.top_log_prob <= 0).all()
+        # One entry: with r the rounding of max k, d = r, s = 2^r and t = r 2^r, so both results are r - log2 s. The
+        # power and the logarithm are off by a step (2^-23) of numbers near 1, t / s by less: 2^-22 and some.
+        assert V > 1 or max(-out.log_prob.min(), out.entropy.max()) <= 2.0 ** -21
+
+
+@gpu
 @pytest.mark.parametrize('V', [18, 300, 9001])
 def test_gpu_temperatures(V):
     logits, index = case((4, ), V, torch.float32, 'cuda')
