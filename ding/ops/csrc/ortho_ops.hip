@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(P::THREADS) product_kernel(
         bm = second_b;
         out = second_out;
     }
-    int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     int wi = wave / (TILE / P::WN) * P::WM, wj = wave % (TILE / P::WN) * P::WN;
     Sums<P> sums;
     auto& acc = sums.acc;
@@ -388,25 +388,40 @@ __global__ void __launch_bounds__(P::THREADS) product_kernel(
 #pragma unroll
         for (int j = 0; j < SJ; ++j) acc[i][j] = (typename M::Acc)(0.f);
 
-    // a wave copies 16 rows of a plane at a time: lane l takes piece l % 4 of row l / 4, from where it belongs
+    // A wave copies 16 rows of a plane at a time: lane l takes piece l % 4 of row l / 4, from where it belongs. What
+    // moves from copy to copy and from stage to stage is the same for all lanes and costs the vector unit nothing.
     constexpr int GROUPS = (PA + PB) * TILE / 16, COPIES = (GROUPS + P::WAVES - 1) / P::WAVES;
+    constexpr int S = P::STAGES, STEPS = kStage / M::DEPTH;
+    int stages = depth / kStage, now = 0, skip = 0;
+    if (kind == SYMMETRIC && gridDim.y > 1) {
+        int each = (stages + gridDim.y - 1) / gridDim.y;
+        skip = min(each * (int)blockIdx.y, stages - 1);
+        stages = max(0, min(each, stages - each * (int)blockIdx.y));
+    }
+    const unsigned own = lane / 4 * kStage + (lane % 4 ^ P::turn(lane / 4)) * 8;
     const _Float16* from[COPIES];
-    int place[COPIES], pitch[COPIES];
+    int64_t step[COPIES];
+    int place[COPIES];
 #pragma unroll
     for (int c = 0; c < COPIES; ++c) {
         int group = min(c * P::WAVES + wave, GROUPS - 1);  // every wave issues as many: some copy the last group again
-        int plane = group / (TILE / 16), first = group % (TILE / 16) * 16, row = first + lane / 4;
-        int piece = (lane % 4) ^ P::turn(row);
+        int plane = group / (TILE / 16), first = group % (TILE / 16) * 16;
         const Split& f = plane < PA ? a : bm;
+        step[c] = (int64_t)f.rows * kStage;
         from[c] = ((plane < PA ? plane : plane - PA) ? f.lo : f.hi) +
-                  f.at(batch, (plane < PA ? bi : bj) * TILE + row, piece * 8);
-        pitch[c] = f.rows;
+                  f.at(batch, (plane < PA ? bi : bj) * TILE + first, 0) + skip * step[c];
         place[c] = plane * P::PLANE + first * kStage;
     }
-    auto fetch = [&](int k0, _Float16* stage) {
+    // The stages in order; behind the last one it copies that again, which nobody reads, so that a wave always has as
+    // many copies on their way.
+    int fetched = 0;
+    auto fetch = [&](_Float16* stage) {
+        bool more = ++fetched < stages;
 #pragma unroll
-        for (int c = 0; c < COPIES; ++c)
-            copy_to_lds(from[c] + (int64_t)k0 * pitch[c], stage + place[c]);
+        for (int c = 0; c < COPIES; ++c) {
+            copy_to_lds(from[c] + own, stage + place[c]);
+            from[c] += more ? step[c] : 0;
+        }
     };
     struct Factors {
         half8 a[PA][SI], b[PB][SJ];
@@ -446,51 +461,48 @@ __global__ void __launch_bounds__(P::THREADS) product_kernel(
     // The factors of the next product are read from LDS while the present ones are multiplied. Copies of a wave arrive
     // in the order of their issue: when only those of the S - 2 later stages are out, the next stage's are there; after
     // the barrier everyone's are, and everyone has read the present stage, which is overwritten then.
-    constexpr int S = P::STAGES, STEPS = kStage / M::DEPTH;
-    int stages = depth / kStage, now = 0;
-    if (kind == SYMMETRIC && gridDim.y > 1) {
-        int each = (stages + gridDim.y - 1) / gridDim.y, skip = each * blockIdx.y;
-        stages = max(0, min(each, stages - skip));
-#pragma unroll
-        for (int c = 0; c < COPIES; ++c) from[c] += (int64_t)skip * kStage * pitch[c];
-    }
     Factors even, odd;
-    auto turn_stage = [&](int k, Factors& f) {
-        if (stages - k >= S)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * COPIES) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (k + S < stages) fetch((k + S) * kStage, lds[now]);
+    auto turn_stage = [&](Factors& f) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S - 2) * COPIES) : "memory");
+        fetch(lds[now]);
         now = now + 1 == S ? 0 : now + 1;
         read(f, lds[now], 0);  // behind the last stage it reads what is there, and nobody uses it
     };
 #pragma unroll
-    for (int k = 0; k < S; ++k)
-        if (k < stages) fetch(k * kStage, lds[k]);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    for (int k = 0; k < S; ++k) fetch(lds[k]);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((S - 1) * COPIES) : "memory");
     read(even, lds[0], 0);
     if constexpr (STEPS == 2) {
         for (int k = 0; k < stages; ++k) {
             read(odd, lds[now], 1);
             multiply(even);
-            turn_stage(k, even);
+            turn_stage(even);
             multiply(odd);
         }
     } else if constexpr (P::TILE == 192) {
         // two sets of factors do not fit in registers beside the sums
         for (int k = 0; k < stages; ++k) {
             multiply(even);
-            turn_stage(k, even);
+            turn_stage(even);
         }
     } else {
-        for (int k = 0; k < stages; k += 2) {
-            turn_stage(k, odd);
+        // pairs of stages without a branch between them: the compiler would move reads behind it, next to their use
+        int k = 0;
+        if (stages % 2) {
+            turn_stage(odd);
             multiply(even);
-            if (k + 1 == stages) break;
-            turn_stage(k + 1, even);
+            even = odd;
+            k = 1;
+        }
+        for (; k < stages; k += 2) {
+            turn_stage(odd);
+            multiply(even);
+            turn_stage(even);
             multiply(odd);
         }
     }
+    // nothing is on its way into LDS when the workgroup gives it back
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
     if (kind == SYMMETRIC && gridDim.y > 1) {
         // a part of the depth: the sums themselves, a quad of a lane side by side with its neighbours'
@@ -829,7 +841,7 @@ struct Plan {
 
 Plan plan_of(int64_t m, int64_t n, int64_t depth, int64_t batch, bool lower, bool single = false) {
     static const struct { int side; double alone, shared; } costs[] = {
-        {256, 5650, 5650}, {192, 4200, 4200}, {128, 2260, 1730}, {96, 1650, 1190}, {64, 900, 640}
+        {256, 5940, 5940}, {192, 3590, 3590}, {128, 1960, 1780}, {96, 1150, 1060}, {64, 680, 570}
     };
     Plan best{0, 1};
     double least = 0;
