@@ -21,10 +21,11 @@
 // taken for results that are rounded to 16 bits, over so many steps that its error stays below a fraction of that
 // rounding (five for bfloat16, three for float16).
 //
-// Large products run at 1.0 to 1.2 PFLOP/s of 16-bit instructions (4096 x 4096 over 8192: 674 us; a library's product of
-// plain half precision reaches 1.3 here, and the instructions alone 1.4 with every unit busy), so a third of that in
-// results; 32-bit library products reach 0.15. What keeps smaller ones lower is LDS, which every tile's factors pass twice, and
-// some 10 us a launch of filling, storing and starting.
+// Large products run at 1.3 PFLOP/s of 16-bit instructions (4096 x 4096 over 8192: 623 us), as a library's product of
+// plain half precision does here, and so at a third of that in results; 32-bit library products reach 0.15. It is the
+// chip's power that bounds them: with zeros for factors the same instructions take a quarter to a third less. Smaller
+// ones are held by LDS, which every tile's factors pass twice, and by 5 to 10 us a launch of filling, storing and
+// starting.
 //
 // All products are "row times row" (C_ij = sum_k A_ik B_jk), which needs X and its transpose: both are kept. Columns are
 // padded with zeros to a multiple of a stage's depth; rows of a tile that lie behind them are memory of ours that may
@@ -832,9 +833,10 @@ int64_t tiles_of(int64_t m, int64_t n, int64_t batch, bool lower, int64_t side) 
 }
 
 // How a product of m x n results (of which the lower triangle, or all) is cut: the tile side, and the parts of its depth.
-// Taken is what has the busiest compute unit done first. Clocks of a stage of two planes, measured: of a tile that has
-// its compute unit to itself, and of one among those that share it; a single plane takes 0.4 of them. Small tiles fill the chip where there are few; large
-// ones need less from memory a product. Parts cost their sums' way through memory and another launch.
+// Taken is what has the busiest compute unit done first. Clocks of a stage of two planes, measured over a depth of 4096:
+// of a tile that has its compute unit to itself, and of one among those that share it; a single plane takes 0.4 of them.
+// Small tiles fill the chip where there are few; large ones need less from memory a product. Parts cost their sums' way
+// through memory and another launch.
 struct Plan {
     int side, parts;
 };
