@@ -17,9 +17,9 @@
 // Two ways through the same polynomial:
 //   direct: G, G G and the product with X every step: m^2 n + m^3 + 2 m^2 n flops (symmetric results by half);
 //   gram:   with Q = a + b G + c G G, P <- Q P and G <- Q G Q, all symmetric, and X <- P X once at the end of some steps.
-// The second is cheaper where n is larger than m, but errors of G grow by a^2 a step where those of X grow by a: it is
-// taken for results that are rounded to 16 bits, over so many steps that its error stays below a fraction of that
-// rounding (five for bfloat16, three for float16).
+// The second is cheaper, but errors of G grow by a^2 a step where those of X grow by a, and a matrix of one dominant
+// direction has its others where such errors come to lie. It is taken for results that are rounded to 16 bits, over so
+// few steps that it loses no more than a factor of four (two, with the usual coefficients).
 //
 // Large products run at 1.3 PFLOP/s of 16-bit instructions (4096 x 4096 over 8192: 623 us), as a library's product of
 // plain half precision does here, and so at a third of that in results; 32-bit library products reach 0.15. It is the
