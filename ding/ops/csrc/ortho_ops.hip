@@ -122,6 +122,10 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(Matrix m, double* __rest
     }
 }
 
+// No matrix but zero takes a larger factor: 2^-149 is the smallest number of 32 bits. With it zero stays zero whatever eps.
+constexpr double kMostFactor = 0x1p200;
+__device__ inline double at_most(double v, double most) { return v > most ? most : v; }  // NaN stays
+
 // X and its transpose from M: a 64 x 64 tile a workgroup, turned in LDS. With `lo` planes X = M scale / (norm + eps);
 // without, X = M times the next lower power of two, exactly, and `rest` takes what is left (in [1, 2)).
 template <typename T>
@@ -139,15 +143,18 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(
     __syncthreads();
     sum = sum_s[0];
     for (int w = 1; w < kThreads / kWave; ++w) sum += sum_s[w];
-    double whole = scale / (sqrt(sum) + eps);
-    float factor = (float)whole, left = 1.f;
+    double whole = at_most(scale / (sqrt(sum) + eps), kMostFactor);
+    float left = 1.f;
     if (!x.lo) {
         int e;
         frexp(whole, &e);
-        // beyond the range of 32 bits the matrix is zero or not finite
-        factor = (float)ldexp(1.0, min(max(e - 1, -120), 120));
-        left = (float)(whole / factor);
+        double power = ldexp(1.0, min(max(e - 1, -300), 300));
+        left = (float)(whole / power);
+        whole = power;
     }
+    // what 32 bits do not hold goes in two steps
+    double near = whole < 0x1p-100 ? 0x1p-100 : at_most(whole, 0x1p100);
+    float factor = (float)near, again = near == whole ? 1.f : (float)(whole / near);
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) rest[b] = left;
     const T* p = (const T*)m.base + b * m.batch_stride;
     int i0 = blockIdx.y * kEdge, j0 = blockIdx.x * kEdge, lane = threadIdx.x % kEdge;
@@ -156,7 +163,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(
     for (int r = threadIdx.x / kEdge; r < kEdge; r += kThreads / kEdge) {
         int i = flip ? lane : r, j = flip ? r : lane;
         bool in = i0 + i < m.rows && j0 + j < m.cols;
-        tile[i][j] = in ? to_f(p[(i0 + i) * m.row_stride + (j0 + j) * m.col_stride]) * factor : 0.f;
+        tile[i][j] = in ? to_f(p[(i0 + i) * m.row_stride + (j0 + j) * m.col_stride]) * factor * again : 0.f;
     }
     __syncthreads();
     // 16 bytes a thread, 1 KB a wave
@@ -627,7 +634,7 @@ __global__ void __launch_bounds__(512) small_kernel(Matrix m, Target to, Small p
     __syncthreads();
     sum = part[0];
     for (int w = 1; w < S::WAVES; ++w) sum += part[w];
-    double factor = p.scale / (sqrt(sum) + p.eps);
+    double factor = at_most(p.scale / (sqrt(sum) + p.eps), kMostFactor);
     // a matrix of numbers below 2^-126 takes a factor that 32 bits do not hold: it goes in two steps
     float first = (float)fmin(factor, 0x1p100), second = (float)(factor / first);
 #pragma unroll

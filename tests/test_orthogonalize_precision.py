@@ -57,3 +57,42 @@ def test_gpu_dominant_direction(m, n, kind, noise, dtype):
     rounding = (want.to(dtype).double() - want).norm()
     off = (orthogonalize(x).double() - want).norm()
     assert off <= 1.02 * rounding + 4e-4 * want.norm(), f"off by {off / want.norm():.3g}"
+
+
+def check_range(device):
+    """Numbers at the ends of their types' ranges, and an eps that is nothing beside any of them."""
+    for dtype, small in ((torch.float32, 1e-37), (torch.float32, 1e-43), (torch.bfloat16, 1e-37), (torch.float16, 1e-6)):
+        for shape in ((20, 30), (200, 300), (3, 90, 140), (300, 200)):
+            zero = torch.zeros(shape, dtype=dtype, device=device)
+            for eps in (1e-7, 1e-38, 1e-100, 5e-324):
+                assert torch.equal(orthogonalize(zero, eps=eps), zero)
+            gen = torch.Generator().manual_seed(0)
+            noise = torch.randn(shape, generator=gen)
+            for scale in (small, torch.finfo(dtype).max / 8):
+                x = (noise * scale).to(dtype).to(device)
+                # a rounding, and 2^-22 * 485 for factors of 22 bits (the lane on the CPU is nearer)
+                want = exact(x, eps=1e-100)
+                allowed = torch.finfo(dtype).eps / 2 + 1.2e-4
+                for eps in (1e-100, 5e-324):
+                    off = (orthogonalize(x, eps=eps).double() - want).norm() / want.norm()
+                    assert off <= allowed, f"{dtype} {shape} {scale} {eps}: off by {off:.3g}"
+
+
+def test_range_cpu():
+    check_range('cpu')
+
+
+@gpu
+def test_gpu_range():
+    check_range('cuda')
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_gpu_largest_norm(dtype):
+    """A norm whose inverse is subnormal in 32 bits."""
+    gen = torch.Generator(device='cuda').manual_seed(0)
+    x = torch.empty(2200, 2100, device='cuda').uniform_(-1, 1, generator=gen).mul_(3e38).to(dtype)
+    want = exact(x)
+    off = (orthogonalize(x).double() - want).norm() / want.norm()
+    assert off <= torch.finfo(dtype).eps / 2 + 1.2e-4, f"off by {off:.3g}"
