@@ -56,6 +56,7 @@ torch::Tensor newton_schulz(
     torch::Tensor matrices, int64_t steps, double a, double b, double c, double eps, std::vector<double> scales,
     int64_t span
 );
+std::vector<std::vector<int64_t>> newton_schulz_plan(int64_t batch, int64_t rows, int64_t cols, bool single);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "DI-engine MI355X HIP kernels (gfx950)";
@@ -79,4 +80,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("gated_linear_recurrence", &gated_linear_recurrence, "gated linear recurrence, with gradient",
           py::call_guard<py::gil_scoped_release>());
     m.def("newton_schulz", &newton_schulz, "orthogonalisation by Newton-Schulz products");
+    m.def("newton_schulz_plan", &newton_schulz_plan, "how newton_schulz cuts its products: [side, parts, workgroups] each");
 }

@@ -802,24 +802,24 @@ __global__ void __launch_bounds__(512) small_kernel(Matrix m, Target to, Small p
                 }
 }
 
-// whether a small kernel takes it; if so it is launched
+// whether one workgroup a matrix of m x n (m <= n) does all of it
+bool small_takes(int64_t m, int64_t n, int64_t batch) {
+    return m <= 128 && n <= 256 && (m <= 64 || n <= 128 || batch >= 16);
+}
+
 template <typename T>
-bool small_run(const Matrix& in, const Target& to, const Small& p, int64_t batch, hipStream_t stream) {
+void small_run(const Matrix& in, const Target& to, const Small& p, int64_t batch, hipStream_t stream) {
     auto go = [&](auto mp, auto np) {
         constexpr int MP = decltype(mp)::value, NP = decltype(np)::value;
         small_kernel<T, MP, NP><<<(unsigned)batch, 512, 0, stream>>>(in, to, p);
-        return true;
     };
-    if (in.rows > 64 && in.cols > 128 && batch < 16) return false;
-    auto wide = [&](auto mp) {
-        if (in.cols <= 64 && decltype(mp)::value == 64) return go(mp, std::integral_constant<int, 64>{});
-        if (in.cols <= 128) return go(mp, std::integral_constant<int, 128>{});
-        if (in.cols <= 256) return go(mp, std::integral_constant<int, 256>{});
-        return false;
-    };
-    if (in.rows <= 64) return wide(std::integral_constant<int, 64>{});
-    if (in.rows <= 128) return wide(std::integral_constant<int, 128>{});
-    return false;
+    auto k64 = std::integral_constant<int, 64>{};
+    auto k128 = std::integral_constant<int, 128>{};
+    auto k256 = std::integral_constant<int, 256>{};
+    if (in.rows <= 64)
+        in.cols <= 64 ? go(k64, k64) : in.cols <= 128 ? go(k64, k128) : go(k64, k256);
+    else
+        in.cols <= 128 ? go(k128, k128) : go(k128, k256);
 }
 
 template <typename F>
@@ -870,6 +870,17 @@ Plan plan_of(int64_t m, int64_t n, int64_t depth, int64_t batch, bool lower, boo
     return best;
 }
 
+// The plans of all products of a call. The symmetric ones: G from X while that has one plane, G, products of m x m
+// matrices, and two of those in one launch; then the product with X, whose depth is never cut.
+struct Plans {
+    Plan first, gram, one, two, update;
+};
+
+Plans plans_of(int64_t m, int64_t n, int64_t batch, bool single) {
+    return {plan_of(m, m, n, batch, true, single), plan_of(m, m, n, batch, true), plan_of(m, m, m, batch, true),
+            plan_of(m, m, m, 2 * batch, true), plan_of(m, n, m, batch, false)};
+}
+
 template <typename F>
 void by_side(int side, int64_t tiles, F&& f) {
     switch (side) {
@@ -904,15 +915,14 @@ torch::Tensor newton_schulz(
                 "orthogonalize: at least one step, fewer than 32768 matrices and sides of up to 2^20");
     double sx = scales[0], sg = scales[1], sb = scales[2], sq = scales[3], sp = scales[4];
     bool one = matrices.scalar_type() != torch::kFloat32;  // X has one plane until it is updated
-    Plan first_plan = plan_of(m, m, n, batch, true, one), gram_plan = plan_of(m, m, n, batch, true);
-    Plan one_plan = plan_of(m, m, m, batch, true), two_plan = plan_of(m, m, m, 2 * batch, true);
+    Plans plan = plans_of(m, n, batch, one);
     const std::pair<Plan, int64_t> plans[] = {
-        {first_plan, batch}, {gram_plan, batch}, {one_plan, batch}, {two_plan, 2 * batch}
+        {plan.first, batch}, {plan.gram, batch}, {plan.one, batch}, {plan.two, 2 * batch}
     };
-    int rect = plan_of(m, n, m, batch, false).side;
+    int rect = plan.update.side;
     // rows that tiles of either side reach, and whole tiles of the packing kernel
     int64_t mp = std::max(up(m, rect), up(m, kEdge)), np = std::max(up(n, rect), up(n, kEdge));
-    for (const auto& [plan, count] : plans) mp = std::max(mp, up(m, plan.side));
+    for (const auto& [p, count] : plans) mp = std::max(mp, up(m, p.side));
     int depth_m = (int)up(m, kStage), depth_n = (int)up(n, kStage);
     Matrix in{matrices.data_ptr(), matrices.stride(0), matrices.stride(tall ? 2 : 1), matrices.stride(tall ? 1 : 2),
               (int)m, (int)n};
@@ -922,13 +932,14 @@ torch::Tensor newton_schulz(
     hipStream_t stream = ding_current_stream();
     Small small{(float)(sg / (sx * sx)), (float)(c * sb / (sg * sg)), (float)(b * sb / sg), (float)(1.0 / sb), (float)a,
                 (float)sx, (float)(1.0 / sx), eps, (int)steps};
-    bool done = false;
-    by_type(matrices, [&](auto* null) {
-        using T = std::remove_pointer_t<decltype(null)>;
-        done = small_run<T>(in, to, small, batch, stream);
-    });
-    HIP_CHECK_LAST();
-    if (done) return result;
+    if (small_takes(m, n, batch)) {
+        by_type(matrices, [&](auto* null) {
+            using T = std::remove_pointer_t<decltype(null)>;
+            small_run<T>(in, to, small, batch, stream);
+        });
+        HIP_CHECK_LAST();
+        return result;
+    }
     auto half = matrices.options().dtype(torch::kFloat16);
     int parts = (int)std::min<int64_t>(kNormBlocks, std::max<int64_t>(1, m * n / (kThreads * 32)));
     auto partial = torch::empty({batch * parts}, matrices.options().dtype(torch::kFloat64));
@@ -952,20 +963,19 @@ torch::Tensor newton_schulz(
         HIP_CHECK_LAST();
     });
     int64_t most = 0;
-    for (const auto& [plan, count] : plans)
-        if (plan.parts > 1)
-            most = std::max(most, tiles_of(m, m, count, true, plan.side) * plan.parts * plan.side * plan.side);
+    for (const auto& [p, count] : plans)
+        if (p.parts > 1) most = std::max(most, tiles_of(m, m, count, true, p.side) * p.parts * p.side * p.side);
     auto sums = torch::empty({most}, matrices.options().dtype(torch::kFloat32));
     float* partial_sums = sums.data_ptr<float>();
     // out = (alpha A B^T + beta E) scaled, for symmetric results; with a second B and out if given
     auto symmetric = [&](Split u, Split v, int depth, Epilogue ep, Split e, Split out, bool single,
                          const Split* v2 = nullptr, const Split* out2 = nullptr) {
         int64_t count = v2 ? 2 * batch : batch;
-        Plan plan = v2 ? two_plan : single ? first_plan : depth == depth_m ? one_plan : gram_plan;
-        by_side(plan.side, tiles_of(m, m, count, true, plan.side) * plan.parts, [&](auto shape) {
+        Plan cut = v2 ? plan.two : single ? plan.first : depth == depth_m ? plan.one : plan.gram;
+        by_side(cut.side, tiles_of(m, m, count, true, cut.side) * cut.parts, [&](auto shape) {
             using P = decltype(shape);
             unsigned r = (unsigned)up(m, P::TILE) / P::TILE, tiles = r * (r + 1) / 2;
-            dim3 grid(tiles, (unsigned)plan.parts, (unsigned)count);
+            dim3 grid(tiles, (unsigned)cut.parts, (unsigned)count);
             auto go = [&](auto kernel) {
                 kernel<<<grid, P::THREADS, 0, stream>>>(u, v, depth, ep, e, out, to, (int)batch, v2 ? *v2 : v,
                                                         out2 ? *out2 : out, partial_sums);
@@ -974,10 +984,10 @@ torch::Tensor newton_schulz(
                 go(product_kernel<P, SYMMETRIC, 1, 1>);
             else
                 go(product_kernel<P, SYMMETRIC, 2, 2>);
-            if (plan.parts > 1) {
+            if (cut.parts > 1) {
                 HIP_CHECK_LAST();
                 join_kernel<P><<<dim3(tiles, 1, (unsigned)count), P::THREADS, 0, stream>>>(
-                    partial_sums, plan.parts, ep, e, out, (int)batch, out2 ? *out2 : out);
+                    partial_sums, cut.parts, ep, e, out, (int)batch, out2 ? *out2 : out);
             }
         });
         HIP_CHECK_LAST();
@@ -1041,4 +1051,18 @@ torch::Tensor newton_schulz(
         update(p[(count + 1) % 2], sp, 0.0, s + count == steps, next);
     }
     return result;
+}
+
+// How newton_schulz cuts the products of a batch: for G of one plane (or as the next where the type has two), G, one and
+// two m x m products and the product with X the tile's side, the parts of the depth and the workgroups. Nothing where a
+// workgroup takes a whole matrix. It needs no device.
+std::vector<std::vector<int64_t>> newton_schulz_plan(int64_t batch, int64_t rows, int64_t cols, bool single) {
+    int64_t m = std::min(rows, cols), n = std::max(rows, cols);
+    if (small_takes(m, n, batch)) return {};
+    Plans p = plans_of(m, n, batch, single);
+    auto row = [&](Plan k, int64_t width, int64_t count, bool lower) -> std::vector<int64_t> {
+        return {k.side, k.parts, tiles_of(m, width, count, lower, k.side) * k.parts};
+    };
+    return {row(p.first, m, batch, true), row(p.gram, m, batch, true), row(p.one, m, batch, true),
+            row(p.two, m, 2 * batch, true), row(p.update, n, batch, false)};
 }

@@ -364,3 +364,11 @@ def newton_schulz(matrices, steps: int, coefficients, eps: float, scales, span: 
     ``span`` 0 keeps the iteration on X, else it runs on G and X is multiplied
     every ``span`` steps."""
     return _load().newton_schulz(matrices, steps, *coefficients, eps, list(scales), span)
+
+
+def newton_schulz_plan(batch: int, rows: int, cols: int, single: bool):
+    """How ``newton_schulz`` cuts the products of such a batch (``single`` for
+    matrices of 16 bits): [tile side, parts of the depth, workgroups] of G in
+    the first step and later, of one and of two products of m x m matrices,
+    and of the product with X. Empty where a workgroup takes a whole matrix."""
+    return _load().newton_schulz_plan(batch, rows, cols, single)
