@@ -32,6 +32,7 @@ constexpr int kMostTop = 32;
 constexpr int64_t kManyRows = 1024;
 constexpr int64_t kFewRows = 256;  // one for each compute unit
 constexpr int kMostJoined = 4096;  // candidates that a row's segments may offer
+constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1024;  // of a launch; more rows than that go in several
 constexpr float kLn2 = 0.69314718055994531f;
 // 2^-200 is zero in 32 bits: entries that far below the maximum count nothing, and 0 * -inf is kept out of the sums
 constexpr float kFar = -200.f;
@@ -211,12 +212,12 @@ __device__ inline void write_nothing(const Out& out, int64_t r, int top, int lan
 // LANES lanes hold a row in registers, PER entries each.
 template <typename T, int LANES, int PER>
 __global__ void __launch_bounds__(kThreads) token_short_fwd(
-    Rows rows, const int64_t* __restrict__ index, Out out, int64_t count, int V, float k, int64_t ignore,
+    Rows rows, const int64_t* __restrict__ index, Out out, int64_t first, int64_t end, int V, float k, int64_t ignore,
     int has_ignore, int top
 ) {
     int lane = threadIdx.x % LANES;
-    int64_t r = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-    if (r >= count) return;
+    int64_t r = first + (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+    if (r >= end) return;
     int64_t token = index[r];
     if (has_ignore && token == ignore) {
         write_nothing(out, r, top, lane, LANES);
@@ -274,11 +275,11 @@ __device__ inline void rank_orders(const unsigned long long* orders, int n, int 
 
 template <typename T, bool TOP, bool ENTROPY, int THREADS>
 __global__ void __launch_bounds__(THREADS) token_segment_fwd(
-    Rows rows, const int64_t* __restrict__ index, Out out, int V, int segments, int length, float k, int64_t ignore,
-    int has_ignore, int top, float* __restrict__ partial, unsigned long long* __restrict__ offered
+    Rows rows, const int64_t* __restrict__ index, Out out, int64_t first, int V, int segments, int length, float k,
+    int64_t ignore, int has_ignore, int top, float* __restrict__ partial, unsigned long long* __restrict__ offered
 ) {
     constexpr int N = Pack<T>::N;
-    int64_t r = blockIdx.x / segments;
+    int64_t r = first + blockIdx.x / segments;
     int seg = blockIdx.x % segments;
     int tid = threadIdx.x;
     int64_t token = index[r];
@@ -402,10 +403,10 @@ __global__ void __launch_bounds__(THREADS) token_segment_fwd(
 // are live: 0.67 ms, 4.8 TB/s, in segments 0.82 ms; 8184 rows of 50001, six tenths live: 102 us against 131).
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads) token_stream_fwd(
-    Rows rows, const int64_t* __restrict__ index, Out out, int V, float k, int64_t ignore, int has_ignore
+    Rows rows, const int64_t* __restrict__ index, Out out, int64_t first, int V, float k, int64_t ignore, int has_ignore
 ) {
     constexpr int N = Pack<T>::N, PACKS = kPerThread / N;
-    int64_t r = blockIdx.x;
+    int64_t r = first + blockIdx.x;
     int tid = threadIdx.x;
     int64_t token = index[r];
     if (has_ignore && token == ignore) {
@@ -477,19 +478,19 @@ __global__ void __launch_bounds__(kThreads) token_stream_fwd(
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_join(
-    Rows rows, const int64_t* __restrict__ index, Out out, int64_t count, int V, int segments, float k,
+    Rows rows, const int64_t* __restrict__ index, Out out, int64_t first, int64_t end, int V, int segments, float k,
     int64_t ignore, int has_ignore, int top, const float* __restrict__ partial,
     const unsigned long long* __restrict__ offered
 ) {
     // with largest entries a workgroup joins one row, else each of its waves does
     int lane = threadIdx.x % kWave;
-    int64_t r = TOP ? blockIdx.x : (int64_t)blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave;
-    if (r >= count) return;
+    int64_t own = TOP ? blockIdx.x : (int64_t)blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave, r = first + own;
+    if (r >= end) return;
     int64_t token = index[r];
     if (has_ignore && token == ignore) return;
     Sums a{-INFINITY, 0.f, 0.f};
     for (int g = lane; g < segments; g += kWave) {
-        const float* p = partial + 3 * (r * segments + g);
+        const float* p = partial + 3 * (own * segments + g);
         a = join(a, Sums{p[0], p[1], p[2]}, k);
     }
     float m = group_max<kWave>(a.m);
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(kThreads) token_join(
     if constexpr (TOP) {
         __shared__ unsigned long long orders[kMostJoined];
         int n = segments * top;
-        for (int i = threadIdx.x; i < n; i += kThreads) orders[i] = offered[r * n + i];
+        for (int i = threadIdx.x; i < n; i += kThreads) orders[i] = offered[own * n + i];
         __syncthreads();
         float log2s = log2_of(a.s);
         rank_orders(orders, n, top, [&](int j, unsigned long long o) { write_top(out, r, top, j, o, a.m, log2s, k); });
@@ -575,12 +576,12 @@ __device__ inline bool own_share(const Grads& g, int64_t r, int top, int j, int6
 
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads) token_short_bwd(
-    Rows rows, const int64_t* __restrict__ index, Grads g, T* __restrict__ grad, int64_t count, int V, float k,
-    float inv_t, int64_t ignore, int has_ignore, int top
+    Rows rows, const int64_t* __restrict__ index, Grads g, T* __restrict__ grad, int64_t first, int64_t end, int V,
+    float k, float inv_t, int64_t ignore, int has_ignore, int top
 ) {
     int lane = threadIdx.x % LANES;
-    int64_t r = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-    if (r >= count) return;
+    int64_t r = first + (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+    if (r >= end) return;
     int64_t token = index[r];
     T* out = grad + r * V;
     if (has_ignore && token == ignore) {
@@ -602,11 +603,11 @@ __global__ void __launch_bounds__(kThreads) token_short_bwd(
 
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads) token_segment_bwd(
-    Rows rows, const int64_t* __restrict__ index, Grads g, T* __restrict__ grad, int V, int segments, int length, float k,
-    float inv_t, int64_t ignore, int has_ignore, int top
+    Rows rows, const int64_t* __restrict__ index, Grads g, T* __restrict__ grad, int64_t first, int V, int segments,
+    int length, float k, float inv_t, int64_t ignore, int has_ignore, int top
 ) {
     constexpr int N = Pack<T>::N;
-    int64_t r = blockIdx.x / segments;
+    int64_t r = first + blockIdx.x / segments;
     int lo = (blockIdx.x % segments) * length, hi = min(V, lo + length);
     int tid = threadIdx.x;
     int64_t token = index[r];
@@ -681,6 +682,16 @@ void check_args(const torch::Tensor& logits, const torch::Tensor& index) {
 // segments of a row are equally long, in whole packs
 int length_of(int V, int segments) { return ((V + segments - 1) / segments + 7) / 8 * 8; }
 
+// go(first, end) for as many rows at a time as a launch holds
+template <typename F>
+void in_launches(int64_t count, int64_t threads_a_row, F&& go) {
+    int64_t most = std::max<int64_t>(1, kMostThreads / threads_a_row);
+    for (int64_t first = 0; first < count; first += most) {
+        go(first, std::min(count, first + most));
+        HIP_CHECK_LAST();
+    }
+}
+
 template <typename F>
 void by_type(const torch::Tensor& x, F&& f) {
     switch (x.scalar_type()) {
@@ -715,7 +726,6 @@ std::vector<torch::Tensor> token_log_prob_fwd(
     auto top_index = top ? torch::empty(tops, opt.dtype(torch::kInt64)) : torch::empty({0}, opt.dtype(torch::kInt64));
     std::vector<torch::Tensor> result{log_prob, entropy, stats, top_log_prob, top_index};
     if (count == 0) return result;
-    TORCH_CHECK(count * segments < (int64_t)1 << 31, "token_log_prob: too many rows");
     Out out{log_prob.data_ptr<float>(), want_entropy ? entropy.data_ptr<float>() : nullptr, stats.data_ptr<float>(),
             top_log_prob.data_ptr<float>(), top_index.data_ptr<int64_t>()};
     float k = (float)(1.4426950408889634 / temperature);
@@ -724,54 +734,61 @@ std::vector<torch::Tensor> token_log_prob_fwd(
     by_type(logits, [&](auto* null) {
         using T = std::remove_pointer_t<decltype(null)>;
         if (V <= 64) {
-            token_short_fwd<T, 16, 4><<<cdiv(count, kThreads / 16), kThreads, 0, stream>>>(
-                rows, ix, out, count, V, k, ignore, has_ignore, top);
+            in_launches(count, 16, [&](int64_t first, int64_t end) {
+                token_short_fwd<T, 16, 4><<<cdiv(end - first, kThreads / 16), kThreads, 0, stream>>>(
+                    rows, ix, out, first, end, V, k, ignore, has_ignore, top);
+            });
         } else if (V <= 512) {
-            token_short_fwd<T, 64, 8><<<cdiv(count, kThreads / 64), kThreads, 0, stream>>>(
-                rows, ix, out, count, V, k, ignore, has_ignore, top);
+            in_launches(count, 64, [&](int64_t first, int64_t end) {
+                token_short_fwd<T, 64, 8><<<cdiv(end - first, kThreads / 64), kThreads, 0, stream>>>(
+                    rows, ix, out, first, end, V, k, ignore, has_ignore, top);
+            });
         } else if (top == 0 && segments > 1 && count >= kManyRows) {
-            if (want_entropy)
-                token_stream_fwd<T, true><<<(unsigned)count, kThreads, 0, stream>>>(rows, ix, out, V, k, ignore, has_ignore);
-            else
-                token_stream_fwd<T, false><<<(unsigned)count, kThreads, 0, stream>>>(rows, ix, out, V, k, ignore, has_ignore);
+            in_launches(count, kThreads, [&](int64_t first, int64_t end) {
+                auto go = [&](auto kernel) {
+                    kernel<<<(unsigned)(end - first), kThreads, 0, stream>>>(rows, ix, out, first, V, k, ignore, has_ignore);
+                };
+                want_entropy ? go(token_stream_fwd<T, true>) : go(token_stream_fwd<T, false>);
+            });
         } else {
-            torch::Tensor partial, offered;
-            float* p = nullptr;
-            unsigned long long* o = nullptr;
-            if (segments > 1) {
-                partial = torch::empty({count * segments * 3}, opt);
-                p = partial.data_ptr<float>();
-                if (top > 0) {
-                    offered = torch::empty({count * segments * top}, opt.dtype(torch::kInt64));
-                    o = (unsigned long long*)offered.data_ptr<int64_t>();
+            int threads = large ? 4 * kThreads : kThreads, length = length_of(V, segments);
+            in_launches(count, (int64_t)segments * threads, [&](int64_t first, int64_t end) {
+                int64_t groups = (end - first) * segments;
+                torch::Tensor partial, offered;
+                float* p = nullptr;
+                unsigned long long* o = nullptr;
+                if (segments > 1) {
+                    partial = torch::empty({groups * 3}, opt);
+                    p = partial.data_ptr<float>();
+                    if (top > 0) {
+                        offered = torch::empty({groups * top}, opt.dtype(torch::kInt64));
+                        o = (unsigned long long*)offered.data_ptr<int64_t>();
+                    }
                 }
-            }
-            dim3 grid((unsigned)(count * segments));
-            int length = length_of(V, segments);
-            auto go = [&](auto kernel) {
-                kernel<<<grid, large ? 4 * kThreads : kThreads, 0, stream>>>(rows, ix, out, V, segments, length, k, ignore,
-                                                                              has_ignore, top, p, o);
-            };
-            if (top > 0)
-                large ? go(token_segment_fwd<T, true, true, 4 * kThreads>) : go(token_segment_fwd<T, true, true, kThreads>);
-            else if (large)
-                go(token_segment_fwd<T, false, true, 4 * kThreads>);
-            else if (want_entropy)
-                go(token_segment_fwd<T, false, true, kThreads>);
-            else
-                go(token_segment_fwd<T, false, false, kThreads>);
-            if (segments > 1) {
-                HIP_CHECK_LAST();
+                auto go = [&](auto kernel) {
+                    kernel<<<(unsigned)groups, threads, 0, stream>>>(rows, ix, out, first, V, segments, length, k, ignore,
+                                                                     has_ignore, top, p, o);
+                };
                 if (top > 0)
-                    token_join<T, true><<<(unsigned)count, kThreads, 0, stream>>>(
-                        rows, ix, out, count, V, segments, k, ignore, has_ignore, top, p, o);
+                    large ? go(token_segment_fwd<T, true, true, 4 * kThreads>) : go(token_segment_fwd<T, true, true, kThreads>);
+                else if (large)
+                    go(token_segment_fwd<T, false, true, 4 * kThreads>);
+                else if (want_entropy)
+                    go(token_segment_fwd<T, false, true, kThreads>);
                 else
-                    token_join<T, false><<<cdiv(count, kThreads / kWave), kThreads, 0, stream>>>(
-                        rows, ix, out, count, V, segments, k, ignore, has_ignore, top, p, o);
-            }
+                    go(token_segment_fwd<T, false, false, kThreads>);
+                if (segments > 1) {
+                    HIP_CHECK_LAST();
+                    if (top > 0)
+                        token_join<T, true><<<(unsigned)(end - first), kThreads, 0, stream>>>(
+                            rows, ix, out, first, end, V, segments, k, ignore, has_ignore, top, p, o);
+                    else
+                        token_join<T, false><<<cdiv(end - first, kThreads / kWave), kThreads, 0, stream>>>(
+                            rows, ix, out, first, end, V, segments, k, ignore, has_ignore, top, p, o);
+                }
+            });
         }
     });
-    HIP_CHECK_LAST();
     return result;
 }
 
@@ -795,7 +812,6 @@ torch::Tensor token_log_prob_bwd(
     };
     auto grad = torch::empty(logits.sizes(), logits.options());
     if (grad.numel() == 0) return grad;
-    TORCH_CHECK(count * segments < (int64_t)1 << 31, "token_log_prob: too many rows");
     Grads g{given(grad_log_prob, count), given(grad_entropy, count), given(grad_top, count * top),
             given(stats, 2 * count), given(entropy, count), top ? top_index.data_ptr<int64_t>() : nullptr};
     TORCH_CHECK(g.stats && (g.h || !g.entropy), "token_log_prob: what the forward pass kept is missing");
@@ -806,20 +822,24 @@ torch::Tensor token_log_prob_bwd(
         using T = std::remove_pointer_t<decltype(null)>;
         T* to = (T*)grad.data_ptr();
         if (V <= 64)
-            token_short_bwd<T, 16><<<cdiv(count, kThreads / 16), kThreads, 0, stream>>>(
-                rows, ix, g, to, count, V, k, inv_t, ignore, has_ignore, top);
+            in_launches(count, 16, [&](int64_t first, int64_t end) {
+                token_short_bwd<T, 16><<<cdiv(end - first, kThreads / 16), kThreads, 0, stream>>>(
+                    rows, ix, g, to, first, end, V, k, inv_t, ignore, has_ignore, top);
+            });
         else if (V <= 512)
-            token_short_bwd<T, 64><<<cdiv(count, kThreads / 64), kThreads, 0, stream>>>(
-                rows, ix, g, to, count, V, k, inv_t, ignore, has_ignore, top);
-        else {
-            auto go = [&](auto kernel) {
-                kernel<<<(unsigned)(count * segments), kThreads, 0, stream>>>(
-                    rows, ix, g, to, V, segments, length_of(V, segments), k, inv_t, ignore, has_ignore, top);
-            };
-            g.entropy ? go(token_segment_bwd<T, true>) : go(token_segment_bwd<T, false>);
-        }
+            in_launches(count, 64, [&](int64_t first, int64_t end) {
+                token_short_bwd<T, 64><<<cdiv(end - first, kThreads / 64), kThreads, 0, stream>>>(
+                    rows, ix, g, to, first, end, V, k, inv_t, ignore, has_ignore, top);
+            });
+        else
+            in_launches(count, (int64_t)segments * kThreads, [&](int64_t first, int64_t end) {
+                auto go = [&](auto kernel) {
+                    kernel<<<(unsigned)((end - first) * segments), kThreads, 0, stream>>>(
+                        rows, ix, g, to, first, V, segments, length_of(V, segments), k, inv_t, ignore, has_ignore, top);
+                };
+                g.entropy ? go(token_segment_bwd<T, true>) : go(token_segment_bwd<T, false>);
+            });
     });
-    HIP_CHECK_LAST();
     return grad;
 }
 

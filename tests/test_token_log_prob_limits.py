@@ -1,0 +1,32 @@
+"""Token log probabilities at the ends of what a call may hold."""
+import pytest
+import torch
+
+from ding.rl_utils import token_log_prob
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize('rows,V,threads', [(2 ** 28 + 70, 2, 16), (2 ** 26 + 37, 66, 64), (2 ** 24 + 5, 513, 256)])
+def test_gpu_more_rows_than_a_launch_holds(rows, V, threads):
+    """A launch takes fewer than 2^32 threads, `threads` of them a row."""
+    assert rows * threads >= 2 ** 32
+    gen = torch.Generator(device='cuda').manual_seed(rows % 1000)
+    logits = torch.empty(rows, V, dtype=torch.bfloat16, device='cuda').normal_(generator=gen).requires_grad_()
+    index = torch.randint(0, V, (rows, ), device='cuda', generator=gen)
+    out = token_log_prob(logits, index, entropy=True)
+    grad, = torch.autograd.grad([out.log_prob.sum() + out.entropy.sum()], [logits])
+    edge = 2 ** 32 // threads
+    parts = [slice(at, at + 100) for at in (0, edge - 150, edge - 50, rows - 100)]
+    parts += [slice(at, at + 4096) for at in range(4096, rows - 4096, rows // 64)]
+    for part in parts:
+        x = logits[part].detach().double()
+        lp = torch.log_softmax(x, -1)
+        p = lp.exp()
+        h = -(p * lp).sum(-1, keepdim=True)
+        want = torch.zeros_like(x).scatter_(-1, index[part].unsqueeze(-1), 1.0) - p - p * (lp + h)
+        # some hundred roundings of 2^-24 of numbers below 16, and the gradient's to 8 bits
+        assert (out.log_prob[part] - lp.gather(-1, index[part].unsqueeze(-1)).squeeze(-1)).abs().max() <= 1e-4
+        assert (out.entropy[part] - h.squeeze(-1)).abs().max() <= 1e-4
+        assert ((grad[part] - want).abs() <= 2.0 ** -8 * want.abs() + 1e-4).all()
