@@ -12,8 +12,9 @@
 // Four ways over the rows, every thread holding 32 logits in registers, so that logits are read once also where the
 // largest are wanted:
 //   up to 512 entries (action sets): 16 or 64 lanes a row, several rows a workgroup;
-//   up to 256 longer rows: segments of up to 32768 logits, 1024 threads each (32 rows of 32000 bf16 with entropy and the
-//   eight largest: 13 us a call, 18 us in segments of 8192);
+//   up to 256 longer rows (and more, where smaller segments offer too many largest entries): segments of up to 32768
+//   logits, 1024 threads each (32 rows of 32000 bf16 with entropy and the eight largest: 13 us a call, 18 us in segments
+//   of 8192);
 //   from 1024 rows on, where no largest are wanted: a workgroup walks a row of its own, see token_stream_fwd;
 //   else equal segments of up to 8192 logits, 256 threads each.
 // The segments of a row are joined by a second, small kernel; a row of one segment needs none.
@@ -711,11 +712,13 @@ std::vector<torch::Tensor> token_log_prob_fwd(
     Rows rows = rows_of(logits);
     int64_t count = index.numel();
     int V = (int)logits.size(-1);
-    // few long rows: four times as many threads hold a segment, which saves the joining launch up to 32768 entries
-    bool large = count <= kFewRows && V > kSegment;
+    // few long rows: four times as many threads hold a segment, which saves the joining launch up to 32768 entries; else
+    // where smaller segments would offer more candidates than the joining kernel holds
+    bool large = V > kSegment && (count <= kFewRows || top * cdiv(V, kSegment) > kMostJoined);
     int segments = cdiv(V, large ? 4 * kSegment : kSegment);
     TORCH_CHECK(top >= 0 && top <= kMostTop && top <= V, "token_log_prob: top_k must be at most ", kMostTop, " and V");
-    TORCH_CHECK(segments == 1 || top * segments <= kMostJoined, "token_log_prob: top_k of ", top, " over ", V, " entries is too much");
+    TORCH_CHECK(segments == 1 || top * segments <= kMostJoined, "token_log_prob: top_k times a row's segments of ",
+                4 * kSegment, " entries must be at most ", kMostJoined, ", got ", top, " over ", V);
     auto opt = logits.options().dtype(torch::kFloat32);
     auto tops = index.sizes().vec();
     tops.push_back(top);

@@ -71,8 +71,9 @@ def token_log_prob(
         - ignore_index (:obj:`Optional[int]`): Rows whose token is this (prompts, padding) are not read: their \
             outputs are 0, their top indexes -1, their gradient 0.
         - entropy (:obj:`bool`): Whether to return the entropy.
-        - top_k (:obj:`int`): The number of most likely tokens to return, at most 32 on a GPU. Among equal logits \
-            the lower index comes first.
+        - top_k (:obj:`int`): The number of most likely tokens to return, on a GPU at most 32, and at most 4096 for \
+            all of a row's parts of 32768 entries (32 of up to 4194304 entries). Among equal logits the lower index \
+            comes first.
     Returns:
         - output (:obj:`namedtuple`): ``log_prob`` [...], ``entropy`` [...], ``top_log_prob`` [..., top_k] in \
             float32 (float64 for float64 logits, which are taken on the CPU only), ``top_index`` [..., top_k] in \
@@ -99,6 +100,9 @@ def token_log_prob(
             raise TypeError(f"logits on a GPU must be float32, bfloat16 or float16, got {logits.dtype}")
         if top_k > 32:
             raise ValueError(f"top_k must be at most 32 on a GPU, got {top_k}")
+        parts = -(-logits.shape[-1] // 32768)
+        if parts > 1 and top_k * parts > 4096:
+            raise ValueError(f"top_k must be at most {4096 // parts} of {logits.shape[-1]} entries on a GPU, got {top_k}")
         return token_log_prob_output(
             *dispatch.token_log_prob(logits, index, temperature, ignore_index, entropy, top_k)
         )

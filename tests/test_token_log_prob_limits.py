@@ -30,3 +30,33 @@ def test_gpu_more_rows_than_a_launch_holds(rows, V, threads):
         assert (out.log_prob[part] - lp.gather(-1, index[part].unsqueeze(-1)).squeeze(-1)).abs().max() <= 1e-4
         assert (out.entropy[part] - h.squeeze(-1)).abs().max() <= 1e-4
         assert ((grad[part] - want).abs() <= 2.0 ** -8 * want.abs() + 1e-4).all()
+
+
+@gpu
+@pytest.mark.parametrize('rows', [3, 256, 257])
+@pytest.mark.parametrize('V,top_k', [(1048577, 32), (1200000, 29)])
+def test_gpu_top_of_long_rows(rows, V, top_k):
+    """How many largest entries a call may ask for goes by the row's length alone, not by the number of rows."""
+    gen = torch.Generator(device='cuda').manual_seed(rows)
+    logits = torch.empty(rows, V, dtype=torch.bfloat16, device='cuda').normal_(generator=gen)
+    index = torch.randint(0, V, (rows, ), device='cuda', generator=gen)
+    out = token_log_prob(logits, index, entropy=True, top_k=top_k)
+    for r in (0, rows // 2, rows - 1):
+        x = logits[r].cpu()
+        order = torch.sort(x.float(), descending=True, stable=True).indices[:top_k]
+        lp = torch.log_softmax(x.double(), -1)
+        assert torch.equal(out.top_index[r].cpu(), order)
+        # a sum of 2^20 terms over 2^10 threads and some hundred roundings of 2^-24 of numbers below 16
+        assert (out.top_log_prob[r].cpu() - lp[order]).abs().max() <= 1e-4
+        assert abs(out.log_prob[r].item() - lp[index[r].item()].item()) <= 1e-4
+        assert abs(out.entropy[r].item() + (lp.exp() * lp).sum().item()) <= 1e-4
+
+
+@gpu
+@pytest.mark.parametrize('rows', [1, 300])
+def test_gpu_too_many_top(rows):
+    logits = torch.zeros(1, 4194305, dtype=torch.bfloat16, device='cuda').expand(rows, -1)
+    index = torch.zeros(rows, dtype=torch.long, device='cuda')
+    with pytest.raises(ValueError, match='31'):
+        token_log_prob(logits, index, top_k=32)
+    assert token_log_prob(logits[:, :4194304], index, top_k=32).top_index[-1].tolist() == list(range(32))
