@@ -886,6 +886,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> token_log
     int64_t top_k
 ) {
     index = index.to(torch::kInt64).contiguous();
+    if (logits.is_cuda() && logits.dim() > 0) rows_of(logits);  // what has to be copied is copied for both directions
     auto out = TokenLogProb::apply(logits, index, temperature, ignore_index.value_or(0), ignore_index.has_value(),
                                    entropy, top_k);
     return {out[0], out[1], out[2], out[3]};

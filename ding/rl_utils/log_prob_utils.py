@@ -64,8 +64,9 @@ def token_log_prob(
         Log probabilities of given tokens, with the distribution's entropy and its most likely tokens if wanted.
         Differentiable with respect to ``logits`` through ``log_prob``, ``entropy`` and ``top_log_prob`` (once).
     Arguments:
-        - logits (:obj:`torch.Tensor`): [..., V] of float32, bfloat16 or float16, of any strides; only a last \
-            dimension that is not dense costs a copy. Entries of ``-inf`` are masked tokens.
+        - logits (:obj:`torch.Tensor`): [..., V] of float32, bfloat16 or float16, of any strides; a copy is \
+            made only where the last dimension is not dense, or the leading ones do not fold into two. Entries of \
+            ``-inf`` are masked tokens.
         - index (:obj:`torch.Tensor`): [...] of integers, the tokens that were taken.
         - temperature (:obj:`float`): The logits are divided by it; in [1e-30, 1e30].
         - ignore_index (:obj:`Optional[int]`): Rows whose token is this (prompts, padding) are not read: their \

@@ -60,3 +60,24 @@ def test_gpu_too_many_top(rows):
     with pytest.raises(ValueError, match='31'):
         token_log_prob(logits, index, top_k=32)
     assert token_log_prob(logits[:, :4194304], index, top_k=32).top_index[-1].tolist() == list(range(32))
+
+
+@gpu
+@pytest.mark.parametrize('V', [300, 9001])
+def test_gpu_one_copy_for_both_directions(V):
+    """Logits that need a copy are copied once: the backward pass makes room for the gradient alone."""
+    gen = torch.Generator(device='cuda').manual_seed(V)
+    index = torch.randint(0, V, (6, 5, 8), device='cuda', generator=gen)
+    apart = torch.randn(6, 5, 8, V, 2, device='cuda', generator=gen)[..., 0]
+    unfolded = torch.randn(12, 10, 16, V, device='cuda', generator=gen)[::2, ::2, ::2]
+    for logits in (apart, unfolded):
+        grads = []
+        for x in (logits.detach(), logits.contiguous()):
+            x.requires_grad_()
+            out = token_log_prob(x, index, entropy=True)
+            total = out.log_prob.sum() + out.entropy.sum()
+            before = torch.cuda.memory_allocated()
+            torch.cuda.reset_peak_memory_stats()
+            grads.append(torch.autograd.grad(total, x)[0])
+            assert torch.cuda.max_memory_allocated() - before < 1.5 * x.numel() * 4
+        assert torch.equal(*grads)
