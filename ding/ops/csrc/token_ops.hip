@@ -10,16 +10,19 @@
 // s = sum 2^d, t = sum 2^d d, so log p = ln2 (d - log2 s) and H = ln2 (log2 s - t / s). All sums are 32 bit.
 //
 // Four ways over the rows, every thread holding 32 logits in registers, so that logits are read once also where the
-// largest are wanted:
-//   up to 512 entries (action sets): 16 or 64 lanes a row, several rows a workgroup;
+// largest are wanted. Times are of bf16 forward calls without the host's part, on both sides of each switch:
+//   up to 512 entries (action sets): 16 lanes a row up to 64 entries, else 64, several rows a workgroup (131072 rows of
+//   64: 11 us with 16 lanes, 42 us with 64; of 512: 73 us, 398 us as segments; 32 rows of 512: 3.9 and 4.6 us);
 //   up to 256 longer rows (and more, where smaller segments offer too many largest entries): segments of up to 32768
-//   logits, 1024 threads each (32 rows of 32000 bf16 with entropy and the eight largest: 13 us a call, 18 us in segments
-//   of 8192);
-//   from 1024 rows on, where no largest are wanted: a workgroup walks a row of its own, see token_stream_fwd;
+//   logits, 1024 threads each. Of 32000 logits with entropy, 256 rows take 8 us and with the eight largest 15 us (10 and
+//   20 us in segments of 8192), 257 rows 12 and 27 us (10 and 24 us), as a compute unit holds one such workgroup. Rows of
+//   65536 entries on without largest ones would be better off in small segments (256 of 131072: 29 us, 24 us);
+//   from 1024 rows on, where no largest are wanted: a workgroup walks a row of its own, see token_stream_fwd (1024 rows of
+//   50001: 25 us, 32 us in segments). It is ahead from 257 rows on already (512 rows of 20000: 7.6 and 10 us);
 //   else equal segments of up to 8192 logits, 256 threads each.
 // The segments of a row are joined by a second, small kernel; a row of one segment needs none.
-// 16384 rows of 131072 bf16 logits, three quarters of them live, take 0.59 ms forward (5.4 TB/s) and 1.33 ms backward
-// (5.6 TB/s); a large copy reaches 4.9 TB/s here.
+// 16384 rows of 131072 bf16 logits, three quarters of them live, take 0.55 to 0.6 ms forward (5.4 TB/s) and 1.33 ms
+// backward (5.6 TB/s); a large copy reaches 4.9 TB/s here.
 #include "common.h"
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -400,8 +403,8 @@ __global__ void __launch_bounds__(THREADS) token_segment_fwd(
 
 // A workgroup walks a whole row, the next 8192 logits on their way while it sums the present ones; each thread keeps
 // sums of its own and moves their reference when it meets a larger logit. For many rows: the chip is full then, and
-// segments of their own would spend their time on starting (16384 rows of 131072 bf16 logits, of which three quarters
-// are live: 0.67 ms, 4.8 TB/s, in segments 0.82 ms; 8184 rows of 50001, six tenths live: 102 us against 131).
+// segments of their own would spend their time on starting (16384 rows of 131072 bf16 logits with entropy, of which three
+// quarters are live: 0.57 ms, in segments 0.76 ms; 8184 rows of 50001, six tenths live: 125 us against 135).
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads) token_stream_fwd(
     Rows rows, const int64_t* __restrict__ index, Out out, int64_t first, int V, float k, int64_t ignore, int has_ignore

@@ -26,7 +26,9 @@ def grpo_policy_error(data: namedtuple, clip_ratio: float = 0.2, beta: float = 0
     """Clipped PPO surrogate per token + beta * k3-KL to a reference policy.
     adv is the per-sequence group-normalized advantage [B]. ``log_prob_fn``
     (logits, action) -> log probabilities: ``fused_method`` reads each logits
-    tensor once on a GPU."""
+    tensor once on a GPU. A function around ``token_log_prob`` may also pass a
+    ``temperature``, or an ``ignore_index`` that marks padding in ``action``:
+    such tokens are not read (``weight`` alone leaves them read)."""
     logit_new, logit_old, logit_ref, action, adv, weight = data
     if weight is None:
         weight = torch.ones_like(action, dtype=logit_new.dtype)
